@@ -9,6 +9,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("GPT_HIP_LIB") or os.path.join(_HERE, "lib", "libgpt_hip.so")   # override: kernel experiments
 
 F32, BF16 = 0, 1
+MXFP8 = 3                       # output of gpt_add_rmsnorm: e4m3 values with a power-of-two scale per 32 columns
 DP_I64, DP_ID_BYTES = 2, 128
 EPI_STORE, EPI_GELU, EPI_RESADD, EPI_STORE_F32, EPI_GELU_AUX, EPI_DGELU, EPI_ACCUM_F32 = range(7)
 MAX_TOKENS = 40
@@ -60,6 +61,35 @@ class PackItem(C.Structure):
 class Workspace(C.Structure):
     _fields_ = [("B_max", i32), ("layer_stride", i32)] + \
                [(n, vp) for n in ("scal", "enc", "x", "h1", "qkv", "att", "h2", "pre", "act", "hf", "stats")]
+
+
+class Dropout(C.Structure):
+    _fields_ = [("p", f64), ("seed", u64), ("offset", u64), ("offset_dev", vp)]
+
+
+class AddRmsNorm(C.Structure):
+    _fields_ = [(n, i32) for n in ("h_dtype", "x_dtype", "y_dtype")] + \
+               [("h", vp), ("ldh", i64), ("resid", vp), ("ldr", i64), ("x_out", vp), ("ldx", i64), ("weight", vp), ("y", vp), ("ldy", i64),
+                ("scales", vp), ("rho", vp), ("rows", i64), ("d", i64), ("eps", f32), ("drop", C.POINTER(Dropout))]
+
+
+class AddRmsNormBwd(C.Structure):
+    _fields_ = [(n, i32) for n in ("h_dtype", "x_dtype", "y_dtype")] + \
+               [("gy", vp), ("ldgy", i64), ("gx", vp), ("ldgx", i64), ("x", vp), ("ldx", i64), ("weight", vp), ("rho", vp),
+                ("dresid", vp), ("lddr", i64), ("dh", vp), ("lddh", i64), ("dweight", vp), ("ws", vp), ("ws_bytes", i64),
+                ("rows", i64), ("d", i64), ("drop", C.POINTER(Dropout))]
+
+
+class DiffAttention(C.Structure):
+    _fields_ = [(n, i32) for n in ("dtype", "B", "Tq", "Tk", "n_head", "hd")] + \
+               [("scale", f32), ("q", vp), ("ldq", i64), ("bsq", i64), ("k", vp), ("ldk", i64), ("bsk", i64), ("v", vp), ("ldv", i64),
+                ("bsv", i64), ("lam", vp), ("lengths", vp), ("out", vp), ("ldo", i64), ("bso", i64), ("lse", vp), ("out2", vp),
+                ("ws", vp), ("ws_bytes", i64)]
+
+
+class DiffAttentionBwd(C.Structure):
+    _fields_ = [("dout", vp), ("lddo", i64), ("bsdo", i64), ("dq", vp), ("lddq", i64), ("bsdq", i64), ("dk", vp), ("lddk", i64),
+                ("bsdk", i64), ("dv", vp), ("lddv", i64), ("bsdv", i64), ("dlam", vp), ("ws", vp), ("ws_bytes", i64)]
 
 
 _PROTOS = {
@@ -131,6 +161,14 @@ _PROTOS = {
                          i32, i32, i32, f32, f32, vp, u64, vp, vp, vp, vp, i32, vp], i32),
     "gpt_ddim_sample_loop": ([C.POINTER(Model), C.POINTER(Workspace), vp, vp, vp, i32, vp, vp, vp, f32, C.POINTER(i64), i32,
                               i32, i32, i32, i32, f32, f32, vp, u64, vp, vp, vp, vp, i32, vp], i32),
+    "gpt_dropout_add": ([i32, vp, i64, i32, vp, i64, vp, i64, i64, i64, C.POINTER(Dropout), vp], i32),
+    "gpt_add_rmsnorm": ([C.POINTER(AddRmsNorm), vp], i32),
+    "gpt_add_rmsnorm_bwd": ([C.POINTER(AddRmsNormBwd), vp], i32),
+    "gpt_add_rmsnorm_bwd_workspace": ([i64, i64, C.POINTER(i64)], i32),
+    "gpt_diff_attention": ([C.POINTER(DiffAttention), vp], i32),
+    "gpt_diff_attention_workspace": ([i32] * 6 + [C.POINTER(i64)], i32),
+    "gpt_diff_attention_bwd": ([C.POINTER(DiffAttention), C.POINTER(DiffAttentionBwd), vp], i32),
+    "gpt_diff_attention_bwd_workspace": ([i32] * 6 + [C.POINTER(i64)], i32),
 }
 
 _lib = None

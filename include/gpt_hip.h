@@ -510,6 +510,119 @@ int gpt_pack_tensors(const gpt_pack_item_t* items, int n_items, int64_t n4, void
  * do not change).  The destinations must not have been written by anyone else in between. */
 int gpt_pack_tensors_if_changed(const gpt_pack_item_t* items, int n_items, int64_t n4, uint64_t* state, void* stream);
 
+/* ---- parts of a differential-attention Block (no counterpart in the reference, except dropout) ---------------------------------
+ * Dropout from a counter-based generator; no mask is stored.  Element i (= row * d + column of the logical [rows, d] tensor) takes
+ * 16 of the 128 bits that Philox4x32-10 gives for counter (i >> 3, offset + *offset_dev) and key seed: word (i & 7) >> 1, the low
+ * half for even i, the high half for odd i.  It is kept iff that number >= thr = round(65536 p), and kept values are multiplied by
+ * 65536 / (65536 - thr): p is realised in steps of 1 / 65536 and the expectation is exact for the realised one (p = 1: all dropped).
+ * Same (seed, offset) = same mask: give every site of a step its own offset.  offset_dev: a device counter (or NULL) added to
+ * offset, read by the kernel - a captured graph whose replays advance it draws new masks; forward and backward of a step must find
+ * the same value there. */
+typedef struct {
+  double p;
+  uint64_t seed, offset;
+  const uint64_t* offset_dev;
+} gpt_dropout_t;
+
+/* out[r, c] (x_dtype) = (resid ? resid[r, c] (x_dtype) : 0) + (kept ? h[r, c] (h_dtype) * 65536 / (65536 - thr) : 0).
+ * Replaces nn.Dropout and the residual addition behind it (Gpt/models/transformer.py:27-28, 50, 66, 70-71).  The gradient of h is
+ * this call on the gradient of out with the same `drop` and resid = NULL; that of resid is the gradient of out itself.
+ * ldh / ldr / ldo: elements from row to row (inputs may have 0); any alignment of whole elements (rows of 16-byte aligned
+ * multiples of 8 elements, or contiguous tensors, take the vector path).  out may be resid or h (same type, same strides).
+ * Dropped elements contribute 0 whatever h holds (NaN and Inf included). */
+int gpt_dropout_add(int h_dtype, const void* h, int64_t ldh, int x_dtype, const void* resid, int64_t ldr, void* out, int64_t ldo,
+                    int64_t rows, int64_t d, const gpt_dropout_t* drop, void* stream);
+
+/* RMS norm of the residual stream, with the residual's addition:
+ *   x[r, c] (x_dtype) = resid[r, c] + drop(h[r, c])                 (h == NULL: x = resid, and x_out is not written)
+ *   rho[r]  (fp32)    = (mean_c x^2 + eps)^-1/2                     (of x as it is stored)
+ *   y[r, c] (y_dtype) = x * rho * weight[c]
+ * y_dtype GPT_F32, GPT_BF16, or GPT_MXFP8: y holds e4m3 (OCP, round to nearest even) values in units of a power-of-two scale per
+ * 32 consecutive columns (d % 32 == 0); scales[r, c / 32] is the scale's biased exponent byte (E8M0: 2^(byte - 127)), the smallest
+ * with amax <= 448 * scale (0 for a block of zeros), so that nothing saturates.  This is the operand layout of the block-scaled
+ * 8-bit matrix instructions.  A NaN in a row makes the row's values NaN. */
+#define GPT_MXFP8 3
+typedef struct {
+  int h_dtype, x_dtype, y_dtype;
+  const void* h;          int64_t ldh;   /* [rows, d] h_dtype, or NULL */
+  const void* resid;      int64_t ldr;   /* [rows, d] x_dtype */
+  void* x_out;            int64_t ldx;   /* [rows, d] x_dtype (may be resid); unused when h == NULL */
+  const float* weight;                   /* [d] */
+  void* y;                int64_t ldy;   /* [rows, d] */
+  uint8_t* scales;                       /* [rows, d / 32] contiguous, GPT_MXFP8 only */
+  float* rho;                            /* [rows], kept for the backward; may be NULL */
+  int64_t rows, d;
+  float eps;
+  const gpt_dropout_t* drop;             /* host pointer; NULL: no dropout */
+} gpt_add_rmsnorm_t;
+int gpt_add_rmsnorm(const gpt_add_rmsnorm_t* a, void* stream);
+
+/* Its backward.  With gy = dL/dy (y_dtype, GPT_F32 or GPT_BF16) and gx = dL/dx_out (x_dtype, NULL: 0):
+ *   dx = gx + rho (weight gy) - x rho^3 mean_c(weight gy x)
+ *   dresid (x_dtype) = dx;   dh (h_dtype) = kept ? dx * 65536 / (65536 - thr) : 0;   dweight[c] (fp32) = sum_r gy x rho
+ * dresid, dh, dweight are stored (not accumulated); dh and dweight may be NULL.  x is the forward's x_out (its resid where h was
+ * NULL).  The sums over rows are taken in a fixed order: the result does not change from run to run.  ws: scratch of
+ * gpt_add_rmsnorm_bwd_workspace(rows, d) bytes, 16-byte aligned, needed when dweight != NULL. */
+typedef struct {
+  int h_dtype, x_dtype, y_dtype;
+  const void* gy;         int64_t ldgy;
+  const void* gx;         int64_t ldgx;
+  const void* x;          int64_t ldx;
+  const float* weight;
+  const float* rho;
+  void* dresid;           int64_t lddr;
+  void* dh;               int64_t lddh;
+  float* dweight;
+  void* ws;               int64_t ws_bytes;
+  int64_t rows, d;
+  const gpt_dropout_t* drop;
+} gpt_add_rmsnorm_bwd_t;
+int gpt_add_rmsnorm_bwd_workspace(int64_t rows, int64_t d, int64_t* host_bytes);
+int gpt_add_rmsnorm_bwd(const gpt_add_rmsnorm_bwd_t* a, void* stream);
+
+/* Differential attention: per head two softmax maps of head dim hd over values of 2 hd, and their difference with a learned weight.
+ * For batch b, head h, map i = 1, 2 (non-causal, as gpt_attention):
+ *   S_i = scale * Q_i K_i^T,  keys >= lengths[b] left out;   P_i = softmax(S_i) over the keys (all 0 where no key is left)
+ *   out = (P_1 - lam[h] P_2) V
+ * q, k, v, out: `dtype`; a token holds n_head * 2 * hd elements: head h's are at columns h * 2 hd .. (q and k: map 1's hd, then map
+ * 2's).  ld* = elements from token to token, bs* = from sample to sample, so that the three may be column ranges of one fused
+ * [B * T, 3 * n_head * 2 * hd] projection.  hd 32, 64, 96 or 128; rows 16-byte aligned.  lam: fp32 [n_head].  lengths: int32
+ * device [B] or NULL (all Tk); values outside [0, Tk] are clamped; what lies in k and v behind a sample's length is never read into
+ * the result (NaN included).  Any Tq, Tk >= 1.  ws: gpt_diff_attention_workspace() bytes of scratch, 16-byte aligned (0 bytes: may
+ * be NULL); calls that overlap in time need a ws each.
+ * For the backward, keep: lse (fp32 [2][B][n_head][Tq], the maps' base-2 log-sum-exp) and out2 (`dtype` [B][Tq][n_head * 2 * hd],
+ * the second map's P_2 V); both NULL where no gradient is wanted. */
+typedef struct {
+  int dtype, B, Tq, Tk, n_head, hd;
+  float scale;
+  const void* q;          int64_t ldq, bsq;
+  const void* k;          int64_t ldk, bsk;
+  const void* v;          int64_t ldv, bsv;
+  const float* lam;
+  const int32_t* lengths;
+  void* out;              int64_t ldo, bso;
+  float* lse;
+  void* out2;
+  void* ws;               int64_t ws_bytes;
+} gpt_diff_attention_t;
+int gpt_diff_attention_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes);
+int gpt_diff_attention(const gpt_diff_attention_t* a, void* stream);
+
+/* Its backward, `f` being the forward's descriptor (out, lse, out2 as it left them).  With dO = dL/dout and dP = dO V^T,
+ * D_i = rowsum(P_i dP), dS_1 = P_1 (dP - D_1), dS_2 = -lam P_2 (dP - D_2):
+ *   dQ_i = scale dS_i K_i,  dK_i = scale dS_i^T Q_i,  dV = (P_1 - lam P_2)^T dO,  dlam[h] = -sum over samples and rows of D_2
+ * All are stored (not accumulated; zeros behind a sample's length), the sums in a fixed order: the same bits on every run. */
+typedef struct {
+  const void* dout;       int64_t lddo, bsdo;
+  void* dq;               int64_t lddq, bsdq;
+  void* dk;               int64_t lddk, bsdk;
+  void* dv;               int64_t lddv, bsdv;
+  float* dlam;                               /* [n_head] */
+  void* ws;               int64_t ws_bytes;  /* gpt_diff_attention_bwd_workspace() bytes, 16-byte aligned */
+} gpt_diff_attention_bwd_t;
+int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes);
+int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_diff_attention_bwd_t* g, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
