@@ -27,6 +27,10 @@ struct Args {
   float* dlam_part;           // [H][B * key tiles]
 };
 
+// Tq, Tk <= 32 (diffattn_short.hip); the backward needs dlam_part [H][B], no lse, out, out2 or delta
+constexpr int SHORT = 32;
+int short_attention(const Args& a, int dtype, int hd, bool backward, hipStream_t s);
+
 __device__ __forceinline__ int valid_keys(const Args& a, int b) {
   if (!a.lengths) return a.Tk;
   const int n = a.lengths[b];

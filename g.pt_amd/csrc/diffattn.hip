@@ -215,6 +215,7 @@ int make_args(const gpt_diff_attention_t* p, const char* who, Args* a) {
 using namespace diffattn;
 
 static int64_t fwd_workspace(int B, int Tq, int Tk, int n_head, int hd) {
+  if (Tq <= SHORT && Tk <= SHORT) return 0;
   const int n = splits_for(B, Tq, Tk, n_head);
   return n > 1 ? (int64_t)n * B * n_head * Tq * (4 * hd + 4) * (int64_t)sizeof(float) : 0;
 }
@@ -230,6 +231,7 @@ extern "C" int gpt_diff_attention(const gpt_diff_attention_t* p, void* stream) {
   const char* who = "gpt_diff_attention";
   Args a;
   if (int st = make_args(p, who, &a)) return st;
+  if (p->Tq <= SHORT && p->Tk <= SHORT) return short_attention(a, p->dtype, p->hd, false, (hipStream_t)stream);
   const int64_t need = fwd_workspace(p->B, p->Tq, p->Tk, p->n_head, p->hd);
   if (need > 0) {
     GPT_REQUIRE(p->ws && (uintptr_t)p->ws % 16 == 0 && p->ws_bytes >= need, "%s: needs %lld bytes of scratch", who, (long long)need);

@@ -224,6 +224,7 @@ int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 using namespace diffattn;
 
 static int64_t bwd_workspace(int B, int Tq, int Tk, int n_head) {
+  if (Tq <= SHORT && Tk <= SHORT) return round16((int64_t)n_head * B * 4);
   return round16((int64_t)2 * B * n_head * Tq * 4) + round16((int64_t)n_head * B * key_tiles(Tk) * 4);
 }
 
@@ -239,7 +240,8 @@ extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_d
   Args a;
   if (int st = make_args(f, who, &a)) return st;
   GPT_REQUIRE(p && p->dout && p->dq && p->dk && p->dv && p->dlam, "%s: null operand", who);
-  GPT_REQUIRE(f->lse && f->out2, "%s: needs the forward's lse and out2", who);
+  const bool is_short = f->Tq <= SHORT && f->Tk <= SHORT;
+  GPT_REQUIRE(is_short || (f->lse && f->out2), "%s: needs the forward's lse and out2", who);
   const int64_t w = (int64_t)f->n_head * 2 * f->hd, es = f->dtype == GPT_BF16 ? 2 : 4;
   auto rows_ok = [&](const void* ptr, int64_t ld, int64_t bs, int T, bool written) {
     return (uintptr_t)ptr % 16 == 0 && (ld * es) % 16 == 0 && (bs * es) % 16 == 0 && bs >= 0 && (T == 1 || ld >= w) && ld < (1 << 25) &&
@@ -254,10 +256,16 @@ extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_d
   a.dq = p->dq; a.lddq = p->lddq; a.bsdq = p->bsdq;
   a.dk = p->dk; a.lddk = p->lddk; a.bsdk = p->bsdk;
   a.dv = p->dv; a.lddv = p->lddv; a.bsdv = p->bsdv;
+  hipStream_t s = (hipStream_t)stream;
+  if (is_short) {
+    a.dlam_part = (float*)p->ws;
+    if (int st = short_attention(a, f->dtype, f->hd, true, s)) return st;
+    hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, (int64_t)a.B, p->dlam);
+    return gpt_launch_status(who);
+  }
   float* delta = (float*)p->ws;
   a.delta = delta;
   a.dlam_part = (float*)((char*)p->ws + round16((int64_t)2 * f->B * f->n_head * f->Tq * 4));
-  hipStream_t s = (hipStream_t)stream;
 #define GO(T)                                          \
   switch (f->hd) {                                     \
     case 32: return launch<T, 32>(a, delta, p->dlam, s);  \

@@ -296,6 +296,9 @@ def rms_norm_mx8(x, weight, eps=1e-5):
 
 
 # ---------------------------------------------------------------------------------------------------- differential attention
+_SHORT = 32     # up to this many queries and keys the backward recomputes the maps and keeps nothing of the forward
+
+
 def _tokens(t, es):
     """`t` [B, T, w] with rows the kernels take (a copy where the strides or the alignment do not allow it): tensor, token and sample stride."""
     B, T, w = t.shape
@@ -340,7 +343,7 @@ def _attention_forward(q, k, v, lam, lengths, n_head, scale, keep):
     with _On(q.device):
         a, held = _attention_struct(q, k, v, lam, lengths, n_head, scale)
         a.out, a.ldo, a.bso = out.data_ptr(), w, Tq * w
-        if keep:
+        if keep and max(a.Tq, a.Tk) > _SHORT:
             lse = torch.empty(2, B, n_head, Tq, dtype=torch.float32, device=q.device)
             out2 = torch.empty_like(out)
             a.lse, a.out2 = lse.data_ptr(), out2.data_ptr()
@@ -364,7 +367,8 @@ def _attention_backward(g, q, k, v, lam, lengths, out, lse, out2, n_head, scale,
         a, held = _attention_struct(q, k, v, lam, lengths, n_head, scale)
         es = q.element_size()
         a.out, a.ldo, a.bso = out.data_ptr(), out.stride(1), out.stride(0)
-        a.lse, a.out2 = lse.data_ptr(), out2.data_ptr()
+        if lse is not None:
+            a.lse, a.out2 = lse.data_ptr(), out2.data_ptr()
         b = L.DiffAttentionBwd()
         g, b.lddo, b.bsdo = _tokens(g, es)
         b.dout = g.data_ptr()

@@ -591,7 +591,8 @@ int gpt_add_rmsnorm_bwd(const gpt_add_rmsnorm_bwd_t* a, void* stream);
  * the result (NaN included).  Any Tq, Tk >= 1.  ws: gpt_diff_attention_workspace() bytes of scratch, 16-byte aligned (0 bytes: may
  * be NULL); calls that overlap in time need a ws each.
  * For the backward, keep: lse (fp32 [2][B][n_head][Tq], the maps' base-2 log-sum-exp) and out2 (`dtype` [B][Tq][n_head * 2 * hd],
- * the second map's P_2 V); both NULL where no gradient is wanted. */
+ * the second map's P_2 V); both NULL where no gradient is wanted, and where Tq and Tk are both <= 32: that backward recomputes the
+ * maps from q and k and needs neither them nor out. */
 typedef struct {
   int dtype, B, Tq, Tk, n_head, hd;
   float scale;
