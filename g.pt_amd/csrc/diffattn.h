@@ -23,7 +23,7 @@ struct Args {
   int64_t lddo, bsdo;
   void *dq, *dk, *dv;
   int64_t lddq, bsdq, lddk, bsdk, lddv, bsdv;
-  const float* delta;         // [2][B][H][Tq]: D_1, D_2
+  const f32x4* stats;         // [B][H][Tq]: lse_1, lse_2, D_1, D_2
   float* dlam_part;           // [H][B * key tiles]
 };
 
@@ -31,81 +31,84 @@ struct Args {
 constexpr int SHORT = 32;
 int short_attention(const Args& a, int dtype, int hd, bool backward, hipStream_t s);
 
+// dynamic LDS beyond 64 KiB has to be granted per kernel and device
+template <typename K>
+static int grant_lds(K kernel, GptPerDevice& once, const char* who) {
+  if (once.here()) return 0;
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+  GPT_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
+  once.here() = true;
+  return 0;
+}
+
 __device__ __forceinline__ int valid_keys(const Args& a, int b) {
   if (!a.lengths) return a.Tk;
   const int n = a.lengths[b];
   return n < 0 ? 0 : n > a.Tk ? a.Tk : n;
 }
 
-// ---- 16 x 16 tiles: an operand fragment is 8 consecutive k-values of one row (row = lane & 15, k = 8 (lane >> 4) + j); the
-// accumulator holds column lane & 15 and rows 4 (lane >> 4) + r.  bf16: one 16x16x32 instruction; fp32: eight 16x16x4 ones, the
-// j-th on the j-th values (any order of k serves as long as both operands use it).
-template <typename T>
-struct Frag;
-template <>
-struct Frag<bf16_t> {
-  bf16x8 v;
-};
-template <>
-struct Frag<float> {
-  float v[8];
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// ---- LDS tiles: rows of 2 hd elements (both maps' halves of q or k, or the values of one head).  16-byte chunk c of row r lies at
+// chunk c ^ f(r): the 16 rows of a ds_read_b128 at one chunk hit 16 different 16-byte bank groups, the 4 rows of a transposing read 4
+// different 64-byte ones.  f has 4 bits where rows start at the same bank (PITCH % 256 == 0), else 3: there bit 3 comes from the row.
+template <typename T, int HD>
+struct Tile {
+  static constexpr int ES = sizeof(T), PITCH = 2 * HD * ES, CPR = PITCH / 16, CM = CPR / 2;   // bytes per row, chunks per row and per map
+  static constexpr int MASK = PITCH % 256 == 0 ? 15 : 7;
+  __device__ static __forceinline__ int f(int r) {
+    if constexpr (PITCH % 256 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
+    return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  }
+  __device__ static __forceinline__ int at(int r, int chunk) { return r * PITCH + ((chunk ^ f(r)) << 4); }
+  // the same in two steps: `base` = at(r, c) of the lane's part c of a chunk number C + c (no common bits), then C
+  __device__ static __forceinline__ int add(int base, int C) { return (base ^ ((C & MASK) << 4)) + ((C & ~MASK) << 4); }
 };
 
-__device__ __forceinline__ void frag_zero(Frag<bf16_t>& f) { f.v = bf16x8{0, 0, 0, 0, 0, 0, 0, 0}; }
-__device__ __forceinline__ void frag_zero(Frag<float>& f) {
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 v;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f.v[j] = 0.f;
+  for (int e = 0; e < 16; ++e) v[e] = 0.f;
+  return v;
 }
-// 8 consecutive elements at p (16-byte aligned), zeros where !ok
-__device__ __forceinline__ Frag<bf16_t> frag_row(const bf16_t* p, bool ok) {
-  Frag<bf16_t> f;
-  frag_zero(f);
-  if (ok) f.v = *reinterpret_cast<const bf16x8*>(p);
-  return f;
-}
-__device__ __forceinline__ Frag<float> frag_row(const float* p, bool ok) {
-  Frag<float> f;
-  frag_zero(f);
-  if (ok) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w; f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
-  }
-  return f;
-}
-// element `col` of the 8 rows that two accumulator tiles of 16 rows give a lane, in their order: row 16 (j >> 2) + 4 g + (j & 3),
-// g = lane >> 4; rows >= n (counted from the tile's first) are zero
+
+// ---- 32 x 32 tiles: the accumulator holds column lane & 31 and rows row_of(register, lane >> 5)
+__device__ __forceinline__ int row_of(int reg, int half) { return (reg & 3) + 8 * (reg >> 2) + 4 * half; }
+
+// acc[row of A][row of B] += one 16-byte chunk of each row per lane half (bf16: 16 k-values, one instruction; fp32: 8, four)
 template <typename T>
-__device__ __forceinline__ Frag<T> frag_column(const T* base, int64_t ld, int g, int n) {
-  Frag<T> f;
+__device__ __forceinline__ f32x16 mma_chunk(const u32x4& a, const u32x4& b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int r = 16 * (j >> 2) + 4 * g + (j & 3);
-    T t = 0;
-    if (r < n) t = base[(int64_t)r * ld];
-    if constexpr (sizeof(T) == 2) f.v[j] = (short)t;
-    else f.v[j] = t;
-  }
-  return f;
-}
-// two accumulator tiles (rows 0..15 and 16..31 of the contraction) as an operand; bf16: rounded once
-__device__ __forceinline__ void frag_from(Frag<bf16_t>& f, const f32x4& lo, const f32x4& hi) {
-  const uint32_t w[4] = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
-  f.v = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
-}
-__device__ __forceinline__ void frag_from(Frag<float>& f, const f32x4& lo, const f32x4& hi) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f.v[j] = lo[j];
-    f.v[4 + j] = hi[j];
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
   }
 }
-__device__ __forceinline__ f32x4 mma16(const Frag<bf16_t>& a, const Frag<bf16_t>& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma16(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
+
+// A 32 x 32 matrix as an operand that contracts over its rows.  bf16: step s, half hh, slot j holds row 16 s + 8 (j >> 2) + 4 hh +
+// (j & 3), which is what an accumulator's registers hold; fp32: register e holds row row_of(e, hh).
+struct Operand {
+  bf16x8 p[2];
+  float f[16];
+};
+template <typename T>
+__device__ __forceinline__ void operand_from(Operand& o, const f32x16& x) {   // bf16: rounded once, here
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
-  return c;
+    for (int s = 0; s < 2; ++s) {
+      u32x4 w;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[8 * s + 2 * j], x[8 * s + 2 * j + 1]);
+      o.p[s] = __builtin_bit_cast(bf16x8, w);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o.f[e] = x[e];
+  }
 }
 
 // 4 consecutive values to memory
@@ -116,14 +119,111 @@ __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32, 1 ulp; exp2(-inf) = 0
 
-// max / sum over the four lanes that hold one accumulator column
-__device__ __forceinline__ float col_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+// ---- tiles shared by a workgroup of NT threads
+// NROWS rows from `src` (row stride ld) by LDS-DMA; rows from `valid` on arrive as zeros (they lie outside the buffer's range).
+// The load is written out because the compiler, which knows the builtin's LDS write, would wait for the tile in flight before every
+// transposing read of the other one.  It has no register result; tile_barrier() waits for it.  (m0, which it sets, is otherwise unused
+// in the kernels that call this: it is the compiler's for LDS-DMA builtins and indexed moves only.)
+template <typename T, int HD, int NROWS, int NT>
+__device__ __forceinline__ void dma_tile(const T* src, int64_t ld, int valid, char* dst, int tid, int wid) {
+  using L = Tile<T, HD>;
+  const int n = valid < NROWS ? valid : NROWS;
+  const uint64_t base = (uint64_t)src;
+  const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((int)(base >> 32)) & 0xffffu,
+                      (uint32_t)__builtin_amdgcn_readfirstlane(n > 0 ? (int)(((int64_t)(n - 1) * ld + 2 * HD) * L::ES) : 0), 0x00020000u};
+  const uint32_t lds = (uint32_t)(uint64_t)(lds_ptr)dst + wid * 1024;
+  constexpr int CHUNKS = NROWS * L::CPR;
+#pragma unroll
+  for (int c0 = 0; c0 < CHUNKS; c0 += NT) {
+    if (CHUNKS % NT != 0 && c0 + wid * 64 >= CHUNKS) break;        // wave-uniform
+    const int ci = c0 + tid, row = ci / L::CPR, pos = ci - row * L::CPR;
+    const uint32_t off = (uint32_t)row * (uint32_t)(ld * L::ES) + (uint32_t)((pos ^ L::f(row)) << 4);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                     __builtin_amdgcn_readfirstlane((int)(lds + c0 * 16))),
+                 "v"(off), "s"(rsrc)
+                 : "memory");
+  }
 }
-__device__ __forceinline__ float col_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+
+// up to 512 consecutive bytes (32 lanes x 16), zeros from `bytes` on
+__device__ __forceinline__ void dma_bytes(const void* src, int bytes, char* dst, int lane) {
+  const uint64_t base = (uint64_t)src;
+  const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((int)(base >> 32)) & 0xffffu,
+                      (uint32_t)__builtin_amdgcn_readfirstlane(bytes < 512 ? bytes : 512), 0x00020000u};
+  if (lane < 32)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                     __builtin_amdgcn_readfirstlane((int)(uint32_t)(uint64_t)(lds_ptr)dst)),
+                 "v"(lane * 16), "s"(rsrc)
+                 : "memory");
 }
+
+// this lane's row of 32 in a tile, as the base that Tile::add takes with an even chunk number C (the lane half reads chunk C + hh)
+template <typename T, int HD>
+__device__ __forceinline__ int row_base(int lane) {
+  return Tile<T, HD>::at(lane & 31, lane >> 5);
+}
+
+// the lane's place in transposed reads of 32 rows x 32 columns (see columns_frag): bf16 reads 4 x 16 blocks (lane group gq = lane >> 4
+// reads rows .. + tq, columns 16 (gq & 1) ..), fp32 single values
+template <typename T, int HD>
+struct ColBase {
+  int lo, hi;
+  __device__ __forceinline__ ColBase(int lane) {
+    using L = Tile<T, HD>;
+    if constexpr (sizeof(T) == 2) {
+      const int gq = lane >> 4, tq = (lane & 15) >> 2, tp = lane & 3, c = 2 * (gq & 1) + (tp >> 1), in = 8 * (tp & 1);
+      lo = L::at(4 * (gq >> 1) + tq, c) + in;
+      hi = L::at(8 + 4 * (gq >> 1) + tq, c) + in;
+    } else {
+      lo = hi = L::at(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
+    }
+  }
+};
+
+// acc[column of the tile][lane's column of X] += sum over rows [row0, row0 + 32) of tile[row][..] X[row][..] for the 32 columns that
+// start at chunk C (a multiple of 4 chunks in bf16, 8 in fp32)
+template <typename T, int HD>
+__device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBase<T, HD>& cb, int row0, int C, const Operand& x, f32x16 acc) {
+  using L = Tile<T, HD>;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const char* p = tile + (row0 + 16 * s) * L::PITCH;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + L::add(cb.lo, C)));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + L::add(cb.hi, C)));
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), x.p[s], acc, 0, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      constexpr int M = L::MASK;                                     // 15: fp32 rows are multiples of 256 bytes
+      const int swz = ((e & 3) << 2) | ((2 * (e >> 2)) & 3);           // f(row_of(e, hh)) = swz ^ hh
+      const char* p = tile + (row0 + (e & 3) + 8 * (e >> 2)) * L::PITCH;
+      const float v = *reinterpret_cast<const float*>(p + (cb.lo ^ (((C ^ swz) & M) << 4)) + ((C & ~M) << 4));
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x.f[e], acc, 0, 0, 0);
+    }
+  }
+  return acc;
+}
+
+// everything this wave has asked of memory and LDS is there, then everyone's is
+template <int LEFT>
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// workgroup -> (pair, block of the pair): all blocks of a (sample, head) on one XCD, whose L2 then holds the rows they share
+__device__ __forceinline__ void xcd_block(int id, int n, int per_pair, int* pair, int* block) {
+  const int q8 = n >> 3, r8 = n & 7, x = id & 7;
+  const int idx = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (id >> 3);
+  *pair = idx / per_pair;
+  *block = idx - *pair * per_pair;
+}
+
+// max / sum over the two lanes that hold one column of a 32 x 32 accumulator
+__device__ __forceinline__ float col_max(float v) { return fmaxf(v, __shfl_xor(v, 32, 64)); }
+__device__ __forceinline__ float col_sum(float v) { return v + __shfl_xor(v, 32, 64); }
 
 }  // namespace diffattn

@@ -1,114 +1,153 @@
 // Differential attention, forward:  out = (softmax(c Q1 K1^T) - lam softmax(c Q2 K2^T)) V   per (sample, head).
-// Stands beside attention.hip (one softmax map, T <= 32).
+// Stands beside attention.hip (one softmax map, T <= 32); diffattn_short.hip takes Tq, Tk <= 32.
 //
-// One sweep over the keys with the running maximum and sum of both softmaxes.  The products are computed transposed,
+// One sweep over the keys with the running maximum and sum of each softmax.  The products are computed transposed,
 //   S^T = K Q^T,   O^T = V^T P^T,
-// so that a lane holds one query's scores (reductions over keys stay in its registers but for two exchanges) and the exponentiated
+// so that a lane holds one query's scores (reductions over keys stay in its registers but for one exchange) and the exponentiated
 // accumulator of S^T is the operand of the second product as it stands.
+// A wave takes 32 queries and ONE map: its accumulator is 32 x 2 hd (128 registers at hd 128) where both maps' would leave one wave
+// per SIMD; the two waves of a query group join their halves through LDS at the end.  K | V tiles of 64 keys (fp32: 32) come by
+// LDS-DMA, double-buffered, one barrier per tile, and serve all waves of the workgroup.
+// The accumulator is rescaled only when a row's maximum has grown by more than a factor of 2^8 over the reference its sums are held
+// against: P stays below 2^8, exact in every format here.
 #include "diffattn.h"
 
 namespace diffattn {
 namespace {
 
-// One wave: 16 queries, both maps; operands straight from global memory.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void fwd_kernel(Args a) {
-  constexpr int KC = HD / 32, CT = 2 * HD / 16;
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int tiles = (a.Tq + 15) / 16, groups = (tiles + 3) / 4;
-  int id = blockIdx.x;
-  const int tile = (id % groups) * 4 + (threadIdx.x >> 6);
-  id /= groups;
-  const int h = id % a.H;
-  id /= a.H;
-  const int b = id % a.B, split = id / a.B;
-  if (tile >= tiles) return;
-  const int len = valid_keys(a, b);
-  const int k0 = split * a.split_keys, k1 = min(len, k0 + a.split_keys);
+constexpr float SLACK = 8.f;   // log2 of the growth that is let pass
+
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
+  using L = Tile<T, HD>;
+  constexpr int NT = NW * 128, KT = sizeof(T) == 2 ? 64 : 32, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];            // [2][K | V]
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), m = wid & 1, grp = wid >> 1;
+  const int blocks = (a.Tq + 32 * NW - 1) / (32 * NW);
+  int pair, rest;
+  xcd_block(blockIdx.x, gridDim.x, blocks * a.splits, &pair, &rest);
+  const int split = rest / blocks, block = rest - split * blocks, b = pair / a.H, h = pair - b * a.H;
+  const int k0 = split * a.split_keys, k1 = min(valid_keys(a, b), k0 + a.split_keys);
   const T* kb = (const T*)a.k + (int64_t)b * a.bsk + h * 2 * HD;
   const T* vb = (const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD;
-  const int qi = tile * 16 + col;
+  const int qi = block * 32 * NW + grp * 32 + r;
   const bool qok = qi < a.Tq;
-  const T* qr = (const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD;
-  Frag<T> qf[2][KC];
+  u32x4 qf[L::CM / 2];
+  {
+    const T* qr = (const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int c = 0; c < KC; ++c) qf[m][c] = frag_row(qr + m * HD + c * 32 + g * 8, qok);
-  f32x4 o[2][CT];
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int t = 0; t < CT; ++t) o[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kt = k0; kt < k1; kt += 32) {
-    Frag<T> pf[2];
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      f32x4 s[2];
-      float mx = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        const int key = kt + 16 * u + col;
-        const T* kr = kb + (int64_t)(key < k1 ? key : k0) * a.ldk + m * HD + g * 8;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) s[u] = mma16(frag_row(kr + c * 32, key < k1), qf[m][c], s[u]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (kt + 16 * u + 4 * g + r >= k1) s[u][r] = -INFINITY;
-          mx = fmaxf(mx, s[u][r]);
-        }
-      }
-      mx = fmaxf(top[m], col_max(mx));                    // finite, or NaN: the tile has a valid key
-      const float ref = mx * a.c2, alpha = exp2_fast(top[m] * a.c2 - ref);
-      top[m] = mx;
-      float part = 0.f;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[u][r] = exp2_fast(s[u][r] * a.c2 - ref);
-          part += s[u][r];
-        }
-      sum[m] = sum[m] * alpha + part;
-#pragma unroll
-      for (int t = 0; t < CT; ++t) o[m][t] *= alpha;
-      frag_from(pf[m], s[0], s[1]);
-    }
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      const Frag<T> vf = frag_column<T>(vb + (int64_t)kt * a.ldv + t * 16 + col, a.ldv, g, k1 - kt);
-#pragma unroll
-      for (int m = 0; m < 2; ++m) o[m][t] = mma16(vf, pf[m], o[m][t]);
+    for (int s = 0; s < L::CM / 2; ++s) {
+      qf[s] = reinterpret_cast<const u32x4*>(qr)[m * L::CM + 2 * s + hh];
+      if (!qok) qf[s] = u32x4{0u, 0u, 0u, 0u};
     }
   }
+  f32x16 o[CT];
 #pragma unroll
-  for (int m = 0; m < 2; ++m) sum[m] = col_sum(sum[m]);
-  if (!qok) return;
+  for (int t = 0; t < CT; ++t) o[t] = zero16();
+  float top = -INFINITY, sum = 0.f;                                       // raw scores; of exp2(c2 (s - top))
+  const int rb = row_base<T, HD>(lane);
+  const ColBase<T, HD> cb(lane);
+  const int n = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+  auto fetch = [&](int it) {
+    const int key = k0 + it * KT;
+    char* dst = smem + (it & 1) * 2 * TILE;
+    dma_tile<T, HD, KT, NT>(kb + (int64_t)key * a.ldk, a.ldk, k1 - key, dst, tid, wid);
+    dma_tile<T, HD, KT, NT>(vb + (int64_t)key * a.ldv, a.ldv, k1 - key, dst + TILE, tid, wid);
+  };
+  if (n > 0) fetch(0);
+  for (int it = 0; it < n; ++it) {
+    tile_barrier<0>();                                                     // tile `it` is here, the other buffer has been read
+    if (it + 1 < n) fetch(it + 1);
+    const char *tk = smem + (it & 1) * 2 * TILE, *tv = tk + TILE;
+    f32x16 s[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) s[u] = zero16();
+#pragma unroll
+    for (int c = 0; c < L::CM / 2; ++c)
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        s[u] = mma_chunk<T>(*reinterpret_cast<const u32x4*>(tk + u * 32 * L::PITCH + L::add(rb, m * L::CM + 2 * c)), qf[c], s[u]);
+    if (k0 + (it + 1) * KT > k1) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (k0 + it * KT + u * 32 + row_of(e, hh) >= k1) s[u][e] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+    mx = col_max(mx);
+    if (__any((mx - top) * a.c2 > SLACK)) {
+      const float now = fmaxf(top, mx), alpha = exp2_fast((top - now) * a.c2);
+      top = now;
+      sum *= alpha;
+#pragma unroll
+      for (int t = 0; t < CT; ++t) o[t] *= alpha;
+    }
+    const float ref = top * a.c2;
+    Operand p[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[u][e] = exp2_fast(s[u][e] * a.c2 - ref);
+        sum += s[u][e];
+      }
+      operand_from<T>(p[u], s[u]);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) o[t] = columns_product<T, HD>(tv, cb, u * 32, t * (32 * L::ES / 16), p[u], o[t]);
+  }
+  sum = col_sum(sum);
   if (a.splits > 1) {
-    float* p = a.part + (((int64_t)split * a.B * a.H + (int64_t)b * a.H + h) * a.Tq + qi) * (4 * HD + 4);
+    if (!qok) return;
+    float* p = a.part + (((int64_t)split * a.B * a.H + pair) * a.Tq + qi) * (4 * HD + 4);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+    for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) store4(p + m * 2 * HD + t * 16 + 4 * g, o[m][t]);
-    if (g == 0) store4(p + 4 * HD, f32x4{top[0], sum[0], top[1], sum[1]});
+      for (int g = 0; g < 4; ++g)
+        store4(p + m * 2 * HD + t * 32 + 8 * g + 4 * hh, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]});
+    if (hh == 0) {
+      p[4 * HD + 2 * m] = top;
+      p[4 * HD + 2 * m + 1] = sum;
+    }
     return;
   }
-  const float lam = a.lam[h];
-  const float inv0 = sum[0] > 0.f ? 1.f / sum[0] : sum[0], inv1 = sum[1] > 0.f ? 1.f / sum[1] : sum[1];   // no key: 0; NaN stays
-  T* orow = (T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD;
-  T* o2 = a.out2 ? (T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD : nullptr;
+  // the second map's wave hands its normalised half over: [t][g] planes of 64 x 16 bytes, the same lane reads what a lane wrote
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;                            // no key: 0; NaN stays
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    const f32x4 second = o[1][t] * inv1;
-    store4(orow + t * 16 + 4 * g, o[0][t] * inv0 - second * lam);
-    if (o2) store4(o2 + t * 16 + 4 * g, second);
+  for (int t = 0; t < CT; ++t) o[t] *= inv;
+  f32x4* ex = reinterpret_cast<f32x4*>(smem) + grp * (CT * 4 * 64) + lane;
+  tile_barrier<0>();
+  if (m == 1) {
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) ex[(t * 4 + g) * 64] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
   }
-  if (a.lse && g == 0) {
+  tile_barrier<0>();
+  if (!qok) return;
+  if (a.lse && hh == 0) a.lse[((int64_t)m * a.B * a.H + pair) * a.Tq + qi] = sum == 0.f ? INFINITY : top * a.c2 + __builtin_amdgcn_logf(sum);
+  if (m == 0) {
+    const float lam = a.lam[h];
+    T* orow = (T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD + 4 * hh;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-      a.lse[(((int64_t)m * a.B + b) * a.H + h) * a.Tq + qi] = sum[m] == 0.f ? INFINITY : top[m] * a.c2 + __builtin_amdgcn_logf(sum[m]);
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        store4(orow + t * 32 + 8 * g, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]} - ex[(t * 4 + g) * 64] * lam);
+  } else if (a.out2) {
+    T* orow = (T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD + 4 * hh;
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) store4(orow + t * 32 + 8 * g, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]});
   }
 }
 
@@ -153,20 +192,36 @@ __global__ __launch_bounds__(256) void combine_kernel(Args a) {
   }
 }
 
-// spans of keys per (sample, head, query tile): as many as fill the chip's 256 CUs with two workgroups each, none shorter than 256 keys
+// query groups of 32 per workgroup: four share a K | V tile where that still leaves every CU a workgroup
+int groups_for(int64_t pairs, int Tq) { return Tq <= 32 ? 1 : pairs * ((Tq + 127) / 128) >= 256 || Tq > 2048 ? 4 : Tq <= 64 ? 2 : 2; }
+
+// spans of keys per (sample, head, query block): as many as give 256 CUs a workgroup each, none shorter than 256 keys
 int splits_for(int B, int Tq, int Tk, int H) {
-  const int64_t wgs = (int64_t)B * H * ((Tq + 63) / 64);
-  if (wgs >= 256) return 1;
-  const int64_t want = (512 + wgs - 1) / wgs, most = (Tk + 255) / 256;
+  const int64_t pairs = (int64_t)B * H;
+  const int nw = groups_for(pairs, Tq);
+  const int64_t wgs = pairs * ((Tq + 32 * nw - 1) / (32 * nw));
+  if (wgs >= 192) return 1;
+  const int64_t want = 256 / wgs, most = (Tk + 255) / 256;
   return (int)(want < most ? want : most);
+}
+
+template <typename T, int HD, int NW>
+int launch_nw(const Args& a, hipStream_t s) {
+  const char* who = "gpt_diff_attention";
+  static GptPerDevice once;
+  if (int st = grant_lds(fwd_kernel<T, HD, NW>, once, who)) return st;
+  const int64_t grid = (int64_t)a.B * a.H * a.splits * ((a.Tq + 32 * NW - 1) / (32 * NW));
+  GPT_REQUIRE(grid * NW * 128 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
+  constexpr int LDS = 4 * (sizeof(T) == 2 ? 64 : 32) * Tile<T, HD>::PITCH;
+  static_assert(NW * 2 * HD / 32 * 4 * 64 * 16 <= LDS, "the hand-over of the second map's halves has to fit the tiles' LDS");
+  hipLaunchKernelGGL((fwd_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 128), LDS, s, a);
+  return gpt_launch_status(who);
 }
 
 template <typename T, int HD>
 int launch(const Args& a, hipStream_t s) {
-  const int64_t groups = ((int64_t)(a.Tq + 15) / 16 + 3) / 4, grid = groups * a.H * a.B * a.splits;
-  GPT_REQUIRE(grid < (1ll << 24), "gpt_diff_attention: too many workgroups (%lld)", (long long)grid);
-  hipLaunchKernelGGL((fwd_kernel<T, HD>), dim3((unsigned)grid), dim3(256), 0, s, a);
-  if (int st = gpt_launch_status("gpt_diff_attention")) return st;
+  const int nw = groups_for((int64_t)a.B * a.H, a.Tq);
+  if (int st = nw == 4 ? launch_nw<T, HD, 4>(a, s) : nw == 2 ? launch_nw<T, HD, 2>(a, s) : launch_nw<T, HD, 1>(a, s)) return st;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.B * a.H * a.Tq;
     hipLaunchKernelGGL((combine_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
@@ -238,7 +293,7 @@ extern "C" int gpt_diff_attention(const gpt_diff_attention_t* p, void* stream) {
     const int n = splits_for(p->B, p->Tq, p->Tk, p->n_head);
     a.part = (float*)p->ws;
     a.splits = n;
-    a.split_keys = ((p->Tk + n - 1) / n + 31) / 32 * 32;
+    a.split_keys = ((p->Tk + n - 1) / n + 63) / 64 * 64;
   }
   hipStream_t s = (hipStream_t)stream;
 #define GO(T)                           \

@@ -14,20 +14,6 @@
 namespace diffattn {
 namespace {
 
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-template <typename T, int HD>
-struct Tile {
-  static constexpr int ES = sizeof(T), PITCH = 2 * HD * ES, CPR = PITCH / 16, CM = CPR / 2;   // bytes per row, chunks per row and per map
-  __device__ static __forceinline__ int f(int r) {
-    if constexpr (PITCH % 256 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
-    return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);               // rows 128 bytes (mod 256) apart: bit 3 comes from the row itself
-  }
-  __device__ static __forceinline__ int at(int r, int chunk) { return r * PITCH + ((chunk ^ f(r)) << 4); }
-};
-
 // rows [0, n) of `src` (row stride ld elements, valid rows: `valid` <= n) to the tile at `dst`; zeros from row `valid` on
 template <typename T, int HD>
 __device__ __forceinline__ void load_tile(const T* src, int64_t ld, int n, int valid, char* dst, int lane) {
@@ -40,25 +26,6 @@ __device__ __forceinline__ void load_tile(const T* src, int64_t ld, int n, int v
     const int ci = c0 + lane, row = ci / L::CPR, pos = ci - row * L::CPR;
     const uint32_t off = (uint32_t)(row * (uint32_t)(ld * L::ES)) + (uint32_t)((pos ^ L::f(row)) << 4);
     if (ci < chunks) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(dst + c0 * 16), 16, off, 0, 0, 0);
-  }
-}
-
-__device__ __forceinline__ f32x16 zero16() {
-  f32x16 v;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) v[e] = 0.f;
-  return v;
-}
-
-// acc[row of A][row of B] += sum over one 16-byte chunk per lane half
-template <typename T>
-__device__ __forceinline__ f32x16 mma_chunk(const u32x4& a, const u32x4& b, f32x16 c) {
-  if constexpr (sizeof(T) == 2) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-    return c;
   }
 }
 
@@ -77,32 +44,8 @@ __device__ __forceinline__ f32x16 rows_product(const char* ta, bool ina, const c
   return acc;
 }
 
-// row of an accumulator register
-__device__ __forceinline__ int row_of(int reg, int half) { return (reg & 3) + 8 * (reg >> 2) + 4 * half; }
-
-// 32 x 32 operand whose contraction index is the 32 rows in the order ORDER: 0 = as an accumulator's registers hold them (step s,
-// half hh, slot j: row 16 s + 8 (j >> 2) + 4 hh + (j & 3)), 1 = ascending (16 s + 8 hh + j)
-struct Operand {
-  bf16x8 p[2];     // bf16
-  float f[16];     // fp32: slot e of half hh: row row_of(e, hh) (order 0) or 2 e + hh (order 1)
-};
-template <typename T>
-__device__ __forceinline__ void operand_from(Operand& o, const f32x16& x) {
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      u32x4 w;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2(x[8 * s + 2 * j], x[8 * s + 2 * j + 1]);
-      o.p[s] = __builtin_bit_cast(bf16x8, w);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o.f[e] = x[e];
-  }
-}
-
-// acc^T[column 32 t + i of the tile][lane's column of X] = sum over the tile's rows (n valid) of tile[row][..] X[row][..]
+// acc^T[column 32 t + i of the tile][lane's column of X] = sum over the tile's rows (n valid) of tile[row][..] X[row][..].  ORDER of the
+// rows in the operand: 0 = an accumulator's (operand_from), 1 = ascending (bf16: 16 s + 8 hh + j; fp32: 2 e + hh)
 template <typename T, int HD, int ORDER>
 __device__ __forceinline__ f32x16 columns_product(const char* tile, int n, int t, const Operand& x, int lane, const char* zero) {
   using L = Tile<T, HD>;
@@ -332,16 +275,6 @@ __global__ __launch_bounds__(64) void short_bwd_kernel(Args a) {
   store_tile<T, HD>((T*)a.dv + (int64_t)b * a.bsdv + h * 2 * HD, a.lddv, a.Tk, tk, lane);
 }
 
-// dynamic LDS beyond 64 KiB has to be granted per kernel and device
-template <typename K>
-int grant(K kernel, GptPerDevice& once, const char* who) {
-  if (once.here()) return 0;
-  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-  GPT_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
-  once.here() = true;
-  return 0;
-}
-
 template <typename T, int HD>
 int go(const Args& a, bool backward, hipStream_t s) {
   using L = Tile<T, HD>;
@@ -349,12 +282,12 @@ int go(const Args& a, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.H));
   if (!backward) {
     const char* who = "gpt_diff_attention";
-    if (int st = grant(short_fwd_kernel<T, HD>, fwd_once, who)) return st;
+    if (int st = grant_lds(short_fwd_kernel<T, HD>, fwd_once, who)) return st;
     hipLaunchKernelGGL((short_fwd_kernel<T, HD>), grid, dim3(64), (a.Tq + 2 * a.Tk) * L::PITCH + 16, s, a);
     return gpt_launch_status(who);
   }
   const char* who = "gpt_diff_attention_bwd";
-  if (int st = grant(short_bwd_kernel<T, HD>, bwd_once, who)) return st;
+  if (int st = grant_lds(short_bwd_kernel<T, HD>, bwd_once, who)) return st;
   const int lds = (2 * a.Tq + a.Tk) * L::PITCH + v_bytes<T, HD>(a.Tk) + 16;
   hipLaunchKernelGGL((short_bwd_kernel<T, HD>), grid, dim3(64), lds, s, a);
   return gpt_launch_status(who);
