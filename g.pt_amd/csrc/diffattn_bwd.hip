@@ -4,16 +4,121 @@
 // The maps are recomputed from the kept log-sum-exps; D_i = dO . O_i comes from the kept outputs.  Two sweeps, over key tiles for dQ
 // and over query tiles for dK / dV, so that every sum is taken by one wave in a fixed order; dlam is summed from the fp32 P_2 and dP
 // of the second sweep (from the rounded outputs it would carry their rounding error).
-// A wave holds 32 rows of its side for BOTH maps - operands and accumulators, up to 450 registers, one wave per SIMD - because dP
-// serves both: a wave per map would compute it twice (a third more matrix work in dQ, a half in dK / dV).  The other side comes in
-// tiles of 32 rows by LDS-DMA, shared by the workgroup's waves; every tile is used twice, by rows for the scores and transposed for
-// the gradient products.
+// A wave holds 16 rows of its side for BOTH maps - operands and accumulators, some 230 registers at hd 128, two waves per SIMD: dP
+// serves both maps, so a wave per map would compute it twice (a third more matrix work in dQ, a half in dK / dV), and 32 rows per wave
+// would leave one wave per SIMD with nothing beside it while it waits for LDS or exponentials (measured at T = 4096, hd 128: dK / dV
+// 1069 us, dQ 735).  The other side comes in tiles of 32 rows by LDS-DMA, shared by the workgroup's waves; every tile is used
+// twice, by rows for the scores and transposed for the gradient products.
 #include "diffattn.h"
 
 namespace diffattn {
 int make_args(const gpt_diff_attention_t* p, const char* who, Args* a);
 
 namespace {
+
+// ---- 16 x 16 tiles: an operand fragment is 8 consecutive k-values of one row (row = lane & 15, k = 8 (lane >> 4) + j); the
+// accumulator holds column lane & 15 and rows 4 (lane >> 4) + r.  bf16: one 16x16x32 instruction; fp32: eight 16x16x4 ones, the
+// j-th on the j-th values (any order of k serves as long as both operands use it).
+template <typename T>
+struct Frag;
+template <>
+struct Frag<bf16_t> {
+  bf16x8 v;
+};
+template <>
+struct Frag<float> {
+  float v[8];
+};
+
+__device__ __forceinline__ void frag_zero(Frag<bf16_t>& f) { f.v = bf16x8{0, 0, 0, 0, 0, 0, 0, 0}; }
+__device__ __forceinline__ void frag_zero(Frag<float>& f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = 0.f;
+}
+// 8 consecutive elements at p (16-byte aligned), zeros where !ok
+__device__ __forceinline__ Frag<bf16_t> frag_row(const bf16_t* p, bool ok) {
+  Frag<bf16_t> f;
+  frag_zero(f);
+  if (ok) f.v = *reinterpret_cast<const bf16x8*>(p);
+  return f;
+}
+__device__ __forceinline__ Frag<float> frag_row(const float* p, bool ok) {
+  Frag<float> f;
+  frag_zero(f);
+  if (ok) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w; f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+  }
+  return f;
+}
+// two accumulator tiles (rows 0..15 and 16..31 of the contraction) as an operand; bf16: rounded once
+__device__ __forceinline__ void frag_from(Frag<bf16_t>& f, const f32x4& lo, const f32x4& hi) {
+  const uint32_t w[4] = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
+  f.v = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+}
+__device__ __forceinline__ void frag_from(Frag<float>& f, const f32x4& lo, const f32x4& hi) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f.v[j] = lo[j];
+    f.v[4 + j] = hi[j];
+  }
+}
+__device__ __forceinline__ f32x4 mma16(const Frag<bf16_t>& a, const Frag<bf16_t>& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma16(const Frag<float>& a, const Frag<float>& b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+
+
+// this lane's row of 16 in a tile: chunk 4 ks + (lane >> 4) in bf16, chunks 8 ks + 2 (lane >> 4) and the next in fp32
+template <typename T, int HD>
+__device__ __forceinline__ int row16_base(int lane) {
+  return Tile<T, HD>::at(lane & 15, sizeof(T) == 2 ? lane >> 4 : 2 * (lane >> 4));
+}
+template <typename T, int HD>
+__device__ __forceinline__ Frag<T> row16(const char* tile, int rb, int row0, int ks) {
+  using L = Tile<T, HD>;
+  Frag<T> f;
+  const char* p = tile + row0 * L::PITCH;                                  // constant but for smem: the instruction's offset
+  if constexpr (sizeof(T) == 2) {
+    f.v = *reinterpret_cast<const bf16x8*>(p + L::add(rb, 4 * ks));
+  } else {
+    const int at = L::add(rb, 8 * ks);
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + at), b = *reinterpret_cast<const f32x4*>(p + (at ^ 16));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
+  }
+  return f;
+}
+
+// columns 16 t .. of a tile of 32 rows as an operand whose contraction index is the rows, in the order in which two accumulator tiles
+// hold them (frag_from): slot j of lane group g = row 16 (j >> 2) + 4 g + (j & 3)
+template <typename T, int HD>
+__device__ __forceinline__ int col16_base(int lane) {
+  using L = Tile<T, HD>;
+  const int g = lane >> 4;
+  if constexpr (sizeof(T) == 2) return L::at(4 * g + ((lane & 15) >> 2), (lane & 3) >> 1) + 8 * (lane & 1);
+  return L::at(4 * g, (lane & 15) >> 2) + (lane & 3) * 4;
+}
+template <typename T, int HD>
+__device__ __forceinline__ Frag<T> col16(const char* tile, int cb, int t) {
+  using L = Tile<T, HD>;
+  Frag<T> f;
+  if constexpr (sizeof(T) == 2) {
+    const char* p = tile + L::add(cb, 2 * t);
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)p);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + 16 * L::PITCH));
+    f.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)                                            // f(row) = ((j & 3) << 2) ^ f(4 g): fp32 rows are multiples of 256 bytes
+      f.v[j] = *reinterpret_cast<const float*>(tile + L::add(cb ^ ((j & 3) << 6), 4 * t) + (16 * (j >> 2) + (j & 3)) * L::PITCH);
+  }
+  return f;
+}
 
 // per (sample, head, query) the two log-sum-exps and D_1 = dO . (out + lam out2), D_2 = dO . out2: 16 lanes each
 template <typename T, int HD>
@@ -58,211 +163,208 @@ __global__ __launch_bounds__(256) void stats_kernel(Args a, f32x4* stats) {
   }
 }
 
-// stages of the tile ring: three where a workgroup has a CU's LDS to itself (the tile after next is in flight while one is used)
+// stages of the tile ring: three where the LDS allows (the tile after next is in flight while one is used)
 template <typename T, int NW>
-constexpr int STAGES = sizeof(T) == 2 && NW == 4 ? 3 : 2;
-// LDS-DMA instructions a wave issues per tile of 32 rows
-template <typename T, int HD, int NW>
-constexpr int DMA_OPS = 32 * Tile<T, HD>::CPR / (NW * 64);
+constexpr int STAGES = sizeof(T) == 2 && NW == 8 ? 3 : 2;
+// The next of NS stages is here.  With three, what was issued after it - two tiles of 32 rows and EXTRA instructions of this wave -
+// may stay in flight.  (The last chunks of a tile may be fewer than the threads: then only the first waves have issued one more.)
+template <typename T, int HD, int NW, int EXTRA>
+__device__ __forceinline__ void stage_barrier(bool more, int wid) {
+  constexpr int CHUNKS = 32 * Tile<T, HD>::CPR, FULL = CHUNKS / (NW * 64), REM = CHUNKS % (NW * 64);
+  if (STAGES<T, NW> < 3 || !more) tile_barrier<0>();
+  else if (REM != 0 && wid * 64 < REM) tile_barrier<2 * (FULL + 1) + EXTRA>();
+  else tile_barrier<2 * FULL + EXTRA>();
+}
 
-// dQ: NW waves of 32 queries; K | V tiles of 32 keys
+// dQ: NW waves of 16 queries; K | V tiles of 32 keys.  S_i^T = K_i Q_i^T and dP^T = V dO^T: keys on the accumulator's rows.
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
   using L = Tile<T, HD>;
-  constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, CT = HD / 32, CC = 32 * L::ES / 16;
+  constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, STAGE = 2 * TILE, KC = HD / 32, CT = HD / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [NS][K | V]
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int blocks = (a.Tq + 32 * NW - 1) / (32 * NW);
+  const int blocks = (a.Tq + 16 * NW - 1) / (16 * NW);
   int pair, block;
   xcd_block(blockIdx.x, gridDim.x, blocks, &pair, &block);
   const int b = pair / a.H, h = pair - b * a.H, len = valid_keys(a, b);
   const T* kb = (const T*)a.k + (int64_t)b * a.bsk + h * 2 * HD;
   const T* vb = (const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD;
-  const int qi = (block * NW + wid) * 32 + r;
+  const int qi = (block * NW + wid) * 16 + col;
   const bool qok = qi < a.Tq;
-  u32x4 qf[L::CPR / 2], gf[L::CPR / 2];
+  Frag<T> qf[2 * KC], gf[2 * KC];
   {
-    const u32x4* qr = reinterpret_cast<const u32x4*>((const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD);
-    const u32x4* gr = reinterpret_cast<const u32x4*>((const T*)a.dout + (int64_t)b * a.bsdo + (int64_t)(qok ? qi : 0) * a.lddo + h * 2 * HD);
+    const T* qr = (const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD + g * 8;
+    const T* gr = (const T*)a.dout + (int64_t)b * a.bsdo + (int64_t)(qok ? qi : 0) * a.lddo + h * 2 * HD + g * 8;
 #pragma unroll
-    for (int s = 0; s < L::CPR / 2; ++s) {
-      qf[s] = qr[2 * s + hh];
-      gf[s] = gr[2 * s + hh];
+    for (int c = 0; c < 2 * KC; ++c) {
+      qf[c] = frag_row(qr + c * 32, qok);
+      gf[c] = frag_row(gr + c * 32, qok);
     }
   }
   const f32x4 st = a.stats[(int64_t)pair * a.Tq + (qok ? qi : 0)];
   const float lam = a.lam[h];
-  f32x16 acc[2][CT];
+  f32x4 acc[2 * CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) acc[0][t] = acc[1][t] = zero16();
-  const int rb = row_base<T, HD>(lane);
-  const ColBase<T, HD> cb(lane);
+  for (int t = 0; t < 2 * CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int rb = row16_base<T, HD>(lane), cb = col16_base<T, HD>(lane);
   const int n = (len + 31) / 32;
-  auto fetch = [&](int it) {
-    char* dst = smem + (it % NS) * 2 * TILE;
+  auto fetch = [&](int it, int at) {
+    char* dst = smem + at;
     dma_tile<T, HD, 32, NT>(kb + (int64_t)it * 32 * a.ldk, a.ldk, len - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(vb + (int64_t)it * 32 * a.ldv, a.ldv, len - it * 32, dst + TILE, tid, wid);
   };
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i)
-    if (i < n) fetch(i);
+    if (i < n) fetch(i, i * STAGE);
+  int now = 0, next = (NS - 1) * STAGE;                                      // stages in use and to be filled
   for (int it = 0; it < n; ++it) {
-    if (NS == 3 && it + 1 < n) tile_barrier<2 * DMA_OPS<T, HD, NW>>();       // tile `it` is here, the next one may be in flight
-    else tile_barrier<0>();
-    if (it + NS - 1 < n) fetch(it + NS - 1);                                 // into the buffer that was read before the barrier
-    const char *tk = smem + (it % NS) * 2 * TILE, *tv = tk + TILE;
-    f32x16 s[2] = {zero16(), zero16()}, dp = zero16();
+    stage_barrier<T, HD, NW, 0>(it + 1 < n, wid);
+    if (it + NS - 1 < n) fetch(it + NS - 1, next);                           // into the buffer that was read before the barrier
+    // the lane's places in this stage, opaque to the compiler: it would keep every variant of them in a register over the loop
+    int rk = rb + now, ck = cb + now;
+    asm volatile("" : "+v"(rk), "+v"(ck));
+    next = now;
+    now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
+    const char *tk = smem, *tv = smem + TILE;
+    f32x4 dp[2], s[2][2];
 #pragma unroll
-    for (int c = 0; c < L::CPR / 2; ++c) {
-      const int m = c >= L::CM / 2;
-      s[m] = mma_chunk<T>(*reinterpret_cast<const u32x4*>(tk + L::add(rb, 2 * c)), qf[c], s[m]);
-      dp = mma_chunk<T>(*reinterpret_cast<const u32x4*>(tv + L::add(rb, 2 * c)), gf[c], dp);
-    }
-    Operand x[2];
-    const bool whole = it * 32 + 32 <= len;
+    for (int u = 0; u < 2; ++u) {
+      dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = exp2_fast(s[m][e] * a.c2 - st[m]), v = p * (dp[e] - st[2 + m]);
-        s[m][e] = whole || it * 32 + row_of(e, hh) < len ? (m ? -lam * v : v) : 0.f;
+      for (int c = 0; c < 2 * KC; ++c) {
+        dp[u] = mma16(row16<T, HD>(tv, rk, 16 * u, c), gf[c], dp[u]);
+        s[c / KC][u] = mma16(row16<T, HD>(tk, rk, 16 * u, c), qf[c], s[c / KC][u]);
       }
-      operand_from<T>(x[m], s[m]);
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) acc[m][t] = columns_product<T, HD>(tk, cb, 0, m * L::CM + t * CC, x[m], acc[m][t]);
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
+          s[m][u][r] = m ? -lam * v : v;
+        }
+    if (it * 32 + 32 > len) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (it * 32 + 16 * u + 4 * g + r >= len) s[m][u][r] = 0.f;
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      Frag<T> x;
+      frag_from(x, s[m][0], s[m][1]);
+#pragma unroll
+      for (int t = 0; t < CT; ++t) acc[m * CT + t] = mma16(col16<T, HD>(tk, ck, m * CT + t), x, acc[m * CT + t]);
+    }
   }
   if (!qok) return;
-  T* dq = (T*)a.dq + (int64_t)b * a.bsdq + (int64_t)qi * a.lddq + h * 2 * HD + 4 * hh;
+  T* dq = (T*)a.dq + (int64_t)b * a.bsdq + (int64_t)qi * a.lddq + h * 2 * HD + 4 * g;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int t = 0; t < CT; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x16& c = acc[m][t];
-        store4(dq + m * HD + t * 32 + 8 * g, f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]} * a.scale);
-      }
+  for (int t = 0; t < 2 * CT; ++t) store4(dq + t * 16, acc[t] * a.scale);
 }
 
-// dK and / or dV: NW waves of 32 keys; Q | dO | statistics tiles of 32 queries.  fp32 at hd 96 and 128 runs the two one after the other: the
-// operands and accumulators of both do not fit a wave's 512 registers.
-enum { WANT_DK = 1, WANT_DV = 2 };
-
-template <typename T, int HD, int NW, int WANT>
+// dK, dV and the tile's share of sum P_2 dP: NW waves of 16 keys; Q | dO | statistics tiles of 32 queries.  S_i = Q_i K_i^T and
+// dP = dO V^T: queries on the accumulator's rows.  Queries behind Tq arrive as zeros in all three: their dP, D and products are 0.
+template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   using L = Tile<T, HD>;
-  constexpr bool DK = (WANT & WANT_DK) != 0, DV = (WANT & WANT_DV) != 0;
-  constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, STAGE = 2 * TILE + 512, CT = HD / 32, CC = 32 * L::ES / 16;
+  constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, STAGE = 2 * TILE + 512, KC = HD / 32, CT = HD / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [NS][Q | dO | stats]
-  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int blocks = (a.Tk + 32 * NW - 1) / (32 * NW);
+  const int blocks = (a.Tk + 16 * NW - 1) / (16 * NW);
   int pair, block;
   xcd_block(blockIdx.x, gridDim.x, blocks, &pair, &block);
   const int b = pair / a.H, h = pair - b * a.H, len = valid_keys(a, b);
   const T* qb = (const T*)a.q + (int64_t)b * a.bsq + h * 2 * HD;
   const T* gb = (const T*)a.dout + (int64_t)b * a.bsdo + h * 2 * HD;
   const f32x4* sb = a.stats + (int64_t)pair * a.Tq;
-  const int key = (block * NW + wid) * 32 + r;
+  const int key = (block * NW + wid) * 16 + col;
   const bool ok = key < len;
-  u32x4 kf[L::CPR / 2], vf[DK ? L::CPR / 2 : 1];
+  Frag<T> kf[2 * KC], vf[2 * KC];
   {
-    const u32x4* kr = reinterpret_cast<const u32x4*>((const T*)a.k + (int64_t)b * a.bsk + (int64_t)(ok ? key : 0) * a.ldk + h * 2 * HD);
-    const u32x4* vr = reinterpret_cast<const u32x4*>((const T*)a.v + (int64_t)b * a.bsv + (int64_t)(ok ? key : 0) * a.ldv + h * 2 * HD);
+    const T* kr = (const T*)a.k + (int64_t)b * a.bsk + (int64_t)(ok ? key : 0) * a.ldk + h * 2 * HD + g * 8;
+    const T* vr = (const T*)a.v + (int64_t)b * a.bsv + (int64_t)(ok ? key : 0) * a.ldv + h * 2 * HD + g * 8;
 #pragma unroll
-    for (int s = 0; s < L::CPR / 2; ++s) {
-      kf[s] = kr[2 * s + hh];
-      if constexpr (DK) vf[s] = vr[2 * s + hh];
+    for (int c = 0; c < 2 * KC; ++c) {
+      kf[c] = frag_row(kr + c * 32, ok);
+      vf[c] = frag_row(vr + c * 32, ok);
     }
   }
   const float lam = a.lam[h];
-  f32x16 dk[2][DK ? CT : 1], dv[DV ? 2 * CT : 1];
+  f32x4 dk[2 * CT], dv[2 * CT];
 #pragma unroll
-  for (int t = 0; t < CT; ++t) {
-    if constexpr (DK) dk[0][t] = dk[1][t] = zero16();
-    if constexpr (DV) dv[t] = dv[CT + t] = zero16();
-  }
+  for (int t = 0; t < 2 * CT; ++t) dk[t] = dv[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   double dlam = 0.0;
-  const int rb = row_base<T, HD>(lane);
-  const ColBase<T, HD> cb(lane);
-  const int n = block * NW * 32 < len ? (a.Tq + 31) / 32 : 0;               // a block without a valid key: zeros
-  auto fetch = [&](int it) {
-    char* dst = smem + (it % NS) * STAGE;
+  const int rb = row16_base<T, HD>(lane), cb = col16_base<T, HD>(lane);
+  const int n = block * NW * 16 < len ? (a.Tq + 31) / 32 : 0;               // a block without a valid key: zeros
+  auto fetch = [&](int it, int at) {
+    char* dst = smem + at;
     dma_tile<T, HD, 32, NT>(qb + (int64_t)it * 32 * a.ldq, a.ldq, a.Tq - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(gb + (int64_t)it * 32 * a.lddo, a.lddo, a.Tq - it * 32, dst + TILE, tid, wid);
     dma_bytes(sb + it * 32, (a.Tq - it * 32) * 16, dst + 2 * TILE, lane);    // every wave the same 512 bytes: one count for all
   };
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i)
-    if (i < n) fetch(i);
+    if (i < n) fetch(i, i * STAGE);
+  int now = 0, next = (NS - 1) * STAGE;
   for (int it = 0; it < n; ++it) {
-    if (NS == 3 && it + 1 < n) tile_barrier<2 * DMA_OPS<T, HD, NW> + 1>();
-    else tile_barrier<0>();
-    if (it + NS - 1 < n) fetch(it + NS - 1);
-    const char *tq = smem + (it % NS) * STAGE, *tg = tq + TILE;
-    const f32x4* ts = reinterpret_cast<const f32x4*>(tg + TILE);
-    f32x16 s[2] = {zero16(), zero16()}, dp = zero16();
-#pragma unroll
-    for (int c = 0; c < L::CPR / 2; ++c) {
-      const int m = c >= L::CM / 2;
-      s[m] = mma_chunk<T>(*reinterpret_cast<const u32x4*>(tq + L::add(rb, 2 * c)), kf[c], s[m]);
-      if constexpr (DK) dp = mma_chunk<T>(*reinterpret_cast<const u32x4*>(tg + L::add(rb, 2 * c)), vf[c], dp);
-    }
-    // queries behind Tq arrive as zeros in Q, dO and the statistics: their dP, D and gradient products are 0
-    f32x16 p;
+    stage_barrier<T, HD, NW, 1>(it + 1 < n, wid);
+    if (it + NS - 1 < n) fetch(it + NS - 1, next);
+    int rq = rb + now, cq = cb + now, sq = 64 * g + now;                     // as in dq_kernel
+    asm volatile("" : "+v"(rq), "+v"(cq), "+v"(sq));
+    next = now;
+    now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
+    const char *tq = smem, *tg = smem + TILE;
+    const f32x4* ts = reinterpret_cast<const f32x4*>(smem + 2 * TILE + sq);
+    f32x4 dp[2], p[2], s[2][2];
     float part = 0.f;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const f32x4 st = ts[row_of(e, hh)];
-      const float p0 = exp2_fast(s[0][e] * a.c2 - st[0]), p1 = exp2_fast(s[1][e] * a.c2 - st[1]);
-      if constexpr (DV) p[e] = p0 - lam * p1;
-      if constexpr (DK) {
-        part += p1 * dp[e];
-        s[0][e] = p0 * (dp[e] - st[2]);
-        s[1][e] = -lam * (p1 * (dp[e] - st[3]));
+    for (int u = 0; u < 2; ++u) {
+      dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2 * KC; ++c) {
+        dp[u] = mma16(row16<T, HD>(tg, rq, 16 * u, c), vf[c], dp[u]);
+        s[c / KC][u] = mma16(row16<T, HD>(tq, rq, 16 * u, c), kf[c], s[c / KC][u]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const f32x4 st = ts[16 * u + r];
+        const float p0 = exp2_fast(s[0][u][r] * a.c2 - st[0]), p1 = exp2_fast(s[1][u][r] * a.c2 - st[1]);
+        p[u][r] = p0 - lam * p1;
+        part += p1 * dp[u][r];
+        s[0][u][r] = p0 * (dp[u][r] - st[2]);
+        s[1][u][r] = -lam * (p1 * (dp[u][r] - st[3]));
       }
     }
     dlam += part;
-    Operand x;
-    if constexpr (DV) {
-      operand_from<T>(x, p);
+    Frag<T> pf, df[2];
+    frag_from(pf, p[0], p[1]);
+    frag_from(df[0], s[0][0], s[0][1]);
+    frag_from(df[1], s[1][0], s[1][1]);
 #pragma unroll
-      for (int t = 0; t < 2 * CT; ++t) dv[t] = columns_product<T, HD>(tg, cb, 0, t * CC, x, dv[t]);
-    }
-    if constexpr (DK) {
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        operand_from<T>(x, s[m]);
-#pragma unroll
-        for (int t = 0; t < CT; ++t) dk[m][t] = columns_product<T, HD>(tq, cb, 0, m * L::CM + t * CC, x, dk[m][t]);
-      }
+    for (int t = 0; t < 2 * CT; ++t) {
+      dv[t] = mma16(col16<T, HD>(tg, cq, t), pf, dv[t]);
+      dk[t] = mma16(col16<T, HD>(tq, cq, t), df[t / CT], dk[t]);
     }
   }
-  if constexpr (DK) {
-    float sum = ok ? (float)dlam : 0.f;
-    sum = wave_sum(sum);
-    if (lane == 0) a.dlam_part[((int64_t)h * a.B + b) * (blocks * NW) + block * NW + wid] = sum;
-  }
+  // a masked key's lane has computed with zeros for its operands and another row's statistics: it gives zeros
+  const float sum = wave_sum(ok ? (float)dlam : 0.f);
+  if (lane == 0) a.dlam_part[((int64_t)h * a.B + b) * (blocks * NW) + block * NW + wid] = sum;
   if (key >= a.Tk) return;
-  // a masked key's lane has computed with another row's operands: it stores zeros
-  auto put = [&](T* row, const f32x16& c, float f) {
+  T* dkr = (T*)a.dk + (int64_t)b * a.bsdk + (int64_t)key * a.lddk + h * 2 * HD + 4 * g;
+  T* dvr = (T*)a.dv + (int64_t)b * a.bsdv + (int64_t)key * a.lddv + h * 2 * HD + 4 * g;
+  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      store4(row + 8 * g, ok ? f32x4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]} * f : f32x4{0.f, 0.f, 0.f, 0.f});
-  };
-  if constexpr (DK) {
-    T* row = (T*)a.dk + (int64_t)b * a.bsdk + (int64_t)key * a.lddk + h * 2 * HD + 4 * hh;
-#pragma unroll
-    for (int t = 0; t < 2 * CT; ++t) put(row + t * 32, dk[t / CT][t % CT], a.scale);
-  }
-  if constexpr (DV) {
-    T* row = (T*)a.dv + (int64_t)b * a.bsdv + (int64_t)key * a.lddv + h * 2 * HD + 4 * hh;
-#pragma unroll
-    for (int t = 0; t < 2 * CT; ++t) put(row + t * 32, dv[t], 1.f);
+  for (int t = 0; t < 2 * CT; ++t) {
+    store4(dkr + t * 16, ok ? dk[t] * a.scale : none);
+    store4(dvr + t * 16, ok ? dv[t] : none);
   }
 }
 
@@ -278,42 +380,35 @@ __global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ par
   if (threadIdx.x == 0) dlam[blockIdx.x] = -((red[0] + red[1]) + (red[2] + red[3]));
 }
 
-// partial sums of dlam per (head, sample): one per 32 keys of the workgroups' blocks
-int64_t key_tiles(int Tk) { return ((int64_t)Tk + 127) / 128 * 4; }
+// partial sums of dlam per (head, sample): one per 16 keys of the workgroups' blocks
+int64_t key_tiles(int Tk) { return ((int64_t)Tk + 127) / 128 * 8; }
 
-// waves of 32 rows per workgroup: four share the tiles where that still gives every CU a workgroup
-int waves_for(int64_t pairs, int T) { return T > 32 && pairs * ((T + 127) / 128) >= 192 ? 4 : 1; }
+// waves of 16 rows per workgroup: eight share the tiles where that still gives every CU a workgroup, else two.  fp32 from hd 96 on:
+// four, which may have 512 registers each (eight would spill)
+template <typename T, int HD>
+constexpr int MANY = sizeof(T) == 4 && HD >= 96 ? 4 : 8;
+bool many_waves(int64_t pairs, int T) { return T > 32 && pairs * ((T + 127) / 128) >= 192; }
 
 template <typename T, int HD, int NW>
 int launch_dq(const Args& a, hipStream_t s) {
   const char* who = "gpt_diff_attention_bwd";
   static GptPerDevice once;
-  const int64_t grid = ((int64_t)a.Tq + 32 * NW - 1) / (32 * NW) * a.H * a.B;
+  const int64_t grid = ((int64_t)a.Tq + 16 * NW - 1) / (16 * NW) * a.H * a.B;
   GPT_REQUIRE(grid * NW * 64 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
   if (int st = grant_lds(dq_kernel<T, HD, NW>, once, who)) return st;
   hipLaunchKernelGGL((dq_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 64), (STAGES<T, NW> * 64 * Tile<T, HD>::PITCH), s, a);
   return gpt_launch_status(who);
 }
 
-template <typename T, int HD, int NW, int WANT>
+template <typename T, int HD, int NW>
 int launch_dkv(const Args& a, hipStream_t s) {
   const char* who = "gpt_diff_attention_bwd";
   static GptPerDevice once;
-  const int64_t grid = ((int64_t)a.Tk + 32 * NW - 1) / (32 * NW) * a.H * a.B;
+  const int64_t grid = ((int64_t)a.Tk + 16 * NW - 1) / (16 * NW) * a.H * a.B;
   GPT_REQUIRE(grid * NW * 64 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
-  if (int st = grant_lds(dkv_kernel<T, HD, NW, WANT>, once, who)) return st;
-  hipLaunchKernelGGL((dkv_kernel<T, HD, NW, WANT>), dim3((unsigned)grid), dim3(NW * 64), (STAGES<T, NW> * (64 * Tile<T, HD>::PITCH + 512)), s, a);
+  if (int st = grant_lds(dkv_kernel<T, HD, NW>, once, who)) return st;
+  hipLaunchKernelGGL((dkv_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 64), (STAGES<T, NW> * (64 * Tile<T, HD>::PITCH + 512)), s, a);
   return gpt_launch_status(who);
-}
-
-template <typename T, int HD, int NW>
-int launch_dkv_all(const Args& a, hipStream_t s) {
-  if constexpr (sizeof(T) == 4 && HD >= 96) {
-    if (int st = launch_dkv<T, HD, NW, WANT_DK>(a, s)) return st;
-    return launch_dkv<T, HD, NW, WANT_DV>(a, s);
-  } else {
-    return launch_dkv<T, HD, NW, WANT_DK | WANT_DV>(a, s);
-  }
 }
 
 template <typename T, int HD>
@@ -323,10 +418,11 @@ int launch(const Args& a, f32x4* stats, float* dlam, hipStream_t s) {
   GPT_REQUIRE(nd < (1ll << 24), "%s: too many rows (%lld)", who, (long long)rows);
   hipLaunchKernelGGL((stats_kernel<T, HD>), dim3((unsigned)nd), dim3(256), 0, s, a, stats);
   if (int st = gpt_launch_status(who)) return st;
-  const int nk = waves_for(pairs, a.Tk);
-  if (int st = nk == 4 ? launch_dkv_all<T, HD, 4>(a, s) : launch_dkv_all<T, HD, 1>(a, s)) return st;
-  if (int st = waves_for(pairs, a.Tq) == 4 ? launch_dq<T, HD, 4>(a, s) : launch_dq<T, HD, 1>(a, s)) return st;
-  const int64_t tiles = ((int64_t)a.Tk + 32 * nk - 1) / (32 * nk) * nk;
+  constexpr int M = MANY<T, HD>;
+  const int nk = many_waves(pairs, a.Tk) ? M : 2;
+  if (int st = nk == M ? launch_dkv<T, HD, M>(a, s) : launch_dkv<T, HD, 2>(a, s)) return st;
+  if (int st = many_waves(pairs, a.Tq) ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, 2>(a, s)) return st;
+  const int64_t tiles = ((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk;
   hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, (int64_t)a.B * tiles, dlam);
   return gpt_launch_status(who);
 }
