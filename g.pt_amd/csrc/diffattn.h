@@ -52,15 +52,20 @@ typedef __attribute__((address_space(3))) v4s* lds_v4s_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // ---- LDS tiles: rows of 2 hd elements (both maps' halves of q or k, or the values of one head).  16-byte chunk c of row r lies at
-// chunk c ^ f(r): the 16 rows of a ds_read_b128 at one chunk hit 16 different 16-byte bank groups, the 4 rows of a transposing read 4
-// different 64-byte ones.  f has 4 bits where rows start at the same bank (PITCH % 256 == 0), else 3: there bit 3 comes from the row.
+// chunk c ^ f(r); f has 4 bits where rows start at the same bank (PITCH % 256 == 0), else 3: there bit 3 comes from the row.  No two
+// lanes that the LDS serves together hit the same bank:
+//   ds_read_b128 serves lanes 0-3, 12-15, 20-27 (measured by its conflicts; the other phases likewise): with one chunk per 32 rows
+//     that is one row of each residue mod 16, with chunk C + (lane >> 4) per 16 rows the quads of rows 0, 3 at chunk C and 1, 2 at
+//     C + 1 - hence quads 1 and 2 in the same half of a 64-byte group;
+//   a transposing read serves 32 lanes: 4 rows x 64 bytes, or 8 rows x 32 (neighbouring quads in different halves).
 template <typename T, int HD>
 struct Tile {
   static constexpr int ES = sizeof(T), PITCH = 2 * HD * ES, CPR = PITCH / 16, CM = CPR / 2;   // bytes per row, chunks per row and per map
   static constexpr int MASK = PITCH % 256 == 0 ? 15 : 7;
   __device__ static __forceinline__ int f(int r) {
-    if constexpr (PITCH % 256 == 0) return ((r & 3) << 2) | ((r >> 2) & 3);
-    return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+    const int b0 = (r >> 2) & 1, b1 = (r >> 3) & 1, pair = ((b0 ^ b1) << 1) | b1;   // quads of rows 0, 1, 2, 3 -> 0, 2, 3, 1
+    if constexpr (PITCH % 256 == 0) return ((r & 3) << 2) | pair;
+    return (((r >> 1) & 1) << 2) | pair;
   }
   __device__ static __forceinline__ int at(int r, int chunk) { return r * PITCH + ((chunk ^ f(r)) << 4); }
   // the same in two steps: `base` = at(r, c) of the lane's part c of a chunk number C + c (no common bits), then C
@@ -197,7 +202,7 @@ __device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBas
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       constexpr int M = L::MASK;                                     // 15: fp32 rows are multiples of 256 bytes
-      const int swz = ((e & 3) << 2) | ((2 * (e >> 2)) & 3);           // f(row_of(e, hh)) = swz ^ hh
+      const int swz = ((e & 3) << 2) | (3 * ((e >> 2) & 1));           // f(row_of(e, hh)) = swz ^ f(4 hh)
       const char* p = tile + (row0 + (e & 3) + 8 * (e >> 2)) * L::PITCH;
       const float v = *reinterpret_cast<const float*>(p + (cb.lo ^ (((C ^ swz) & M) << 4)) + ((C & ~M) << 4));
       acc = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x.f[e], acc, 0, 0, 0);

@@ -35,19 +35,21 @@ __device__ __forceinline__ void frag_zero(Frag<float>& f) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) f.v[j] = 0.f;
 }
-// 8 consecutive elements at p (16-byte aligned), zeros where !ok
-__device__ __forceinline__ Frag<bf16_t> frag_row(const bf16_t* p, bool ok) {
+// block c of 32 elements of the row at p (16-byte aligned), zeros where !ok: lane group g takes 8 consecutive ones in bf16, two
+// 16-byte chunks four apart in fp32 (as row16 reads them)
+__device__ __forceinline__ Frag<bf16_t> frag_row(const bf16_t* p, int c, int g, bool ok) {
   Frag<bf16_t> f;
   frag_zero(f);
-  if (ok) f.v = *reinterpret_cast<const bf16x8*>(p);
+  if (ok) f.v = *reinterpret_cast<const bf16x8*>(p + c * 32 + g * 8);
   return f;
 }
-__device__ __forceinline__ Frag<float> frag_row(const float* p, bool ok) {
+__device__ __forceinline__ Frag<float> frag_row(const float* p, int c, int g, bool ok) {
   Frag<float> f;
   frag_zero(f);
   if (ok) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f.v[0] = a.x; f.v[1] = a.y; f.v[2] = a.z; f.v[3] = a.w; f.v[4] = b.x; f.v[5] = b.y; f.v[6] = b.z; f.v[7] = b.w;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + c * 32 + g * 4), b = *reinterpret_cast<const f32x4*>(p + c * 32 + 16 + g * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
   }
   return f;
 }
@@ -73,10 +75,10 @@ __device__ __forceinline__ f32x4 mma16(const Frag<float>& a, const Frag<float>& 
 }
 
 
-// this lane's row of 16 in a tile: chunk 4 ks + (lane >> 4) in bf16, chunks 8 ks + 2 (lane >> 4) and the next in fp32
+// this lane's row of 16 in a tile: chunk 4 ks + (lane >> 4) in bf16, chunks 8 ks + (lane >> 4) and four further in fp32
 template <typename T, int HD>
 __device__ __forceinline__ int row16_base(int lane) {
-  return Tile<T, HD>::at(lane & 15, sizeof(T) == 2 ? lane >> 4 : 2 * (lane >> 4));
+  return Tile<T, HD>::at(lane & 15, lane >> 4);
 }
 template <typename T, int HD>
 __device__ __forceinline__ Frag<T> row16(const char* tile, int rb, int row0, int ks) {
@@ -86,8 +88,7 @@ __device__ __forceinline__ Frag<T> row16(const char* tile, int rb, int row0, int
   if constexpr (sizeof(T) == 2) {
     f.v = *reinterpret_cast<const bf16x8*>(p + L::add(rb, 4 * ks));
   } else {
-    const int at = L::add(rb, 8 * ks);
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p + at), b = *reinterpret_cast<const f32x4*>(p + (at ^ 16));
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p + L::add(rb, 8 * ks)), b = *reinterpret_cast<const f32x4*>(p + L::add(rb, 8 * ks + 4));
 #pragma unroll
     for (int j = 0; j < 4; ++j) { f.v[j] = a[j]; f.v[4 + j] = b[j]; }
   }
@@ -194,12 +195,12 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
   const bool qok = qi < a.Tq;
   Frag<T> qf[2 * KC], gf[2 * KC];
   {
-    const T* qr = (const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD + g * 8;
-    const T* gr = (const T*)a.dout + (int64_t)b * a.bsdo + (int64_t)(qok ? qi : 0) * a.lddo + h * 2 * HD + g * 8;
+    const T* qr = (const T*)a.q + (int64_t)b * a.bsq + (int64_t)(qok ? qi : 0) * a.ldq + h * 2 * HD;
+    const T* gr = (const T*)a.dout + (int64_t)b * a.bsdo + (int64_t)(qok ? qi : 0) * a.lddo + h * 2 * HD;
 #pragma unroll
     for (int c = 0; c < 2 * KC; ++c) {
-      qf[c] = frag_row(qr + c * 32, qok);
-      gf[c] = frag_row(gr + c * 32, qok);
+      qf[c] = frag_row(qr, c, g, qok);
+      gf[c] = frag_row(gr, c, g, qok);
     }
   }
   const f32x4 st = a.stats[(int64_t)pair * a.Tq + (qok ? qi : 0)];
@@ -289,12 +290,12 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   const bool ok = key < len;
   Frag<T> kf[2 * KC], vf[2 * KC];
   {
-    const T* kr = (const T*)a.k + (int64_t)b * a.bsk + (int64_t)(ok ? key : 0) * a.ldk + h * 2 * HD + g * 8;
-    const T* vr = (const T*)a.v + (int64_t)b * a.bsv + (int64_t)(ok ? key : 0) * a.ldv + h * 2 * HD + g * 8;
+    const T* kr = (const T*)a.k + (int64_t)b * a.bsk + (int64_t)(ok ? key : 0) * a.ldk + h * 2 * HD;
+    const T* vr = (const T*)a.v + (int64_t)b * a.bsv + (int64_t)(ok ? key : 0) * a.ldv + h * 2 * HD;
 #pragma unroll
     for (int c = 0; c < 2 * KC; ++c) {
-      kf[c] = frag_row(kr + c * 32, ok);
-      vf[c] = frag_row(vr + c * 32, ok);
+      kf[c] = frag_row(kr, c, g, ok);
+      vf[c] = frag_row(vr, c, g, ok);
     }
   }
   const float lam = a.lam[h];
