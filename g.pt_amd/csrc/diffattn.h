@@ -136,16 +136,23 @@ __device__ __forceinline__ void dma_tile(const T* src, int64_t ld, int valid, ch
   const uint64_t base = (uint64_t)src;
   const u32x4 rsrc = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)base), (uint32_t)__builtin_amdgcn_readfirstlane((int)(base >> 32)) & 0xffffu,
                       (uint32_t)__builtin_amdgcn_readfirstlane(n > 0 ? (int)(((int64_t)(n - 1) * ld + 2 * HD) * L::ES) : 0), 0x00020000u};
-  const uint32_t lds = (uint32_t)(uint64_t)(lds_ptr)dst + wid * 1024;
-  constexpr int CHUNKS = NROWS * L::CPR;
+  const uint32_t lds = (uint32_t)(uint64_t)(lds_ptr)dst + wid * 1024, row_bytes = (uint32_t)(ld * L::ES);
+  constexpr int CHUNKS = NROWS * L::CPR, STEP = NT / L::CPR;
+  // threads NT chunks apart: whole rows apart where NT is a multiple of a row's chunks, at the same swizzle where of 16 rows'
+  constexpr bool EVEN = NT % (16 * L::CPR) == 0;
+  asm volatile("" : "+v"(tid));                                    // the offset is formed anew each time: no register over the loop
+  uint32_t off = 0;
 #pragma unroll
   for (int c0 = 0; c0 < CHUNKS; c0 += NT) {
     if (CHUNKS % NT != 0 && c0 + wid * 64 >= CHUNKS) break;        // wave-uniform
-    const int ci = c0 + tid, row = ci / L::CPR, pos = ci - row * L::CPR;
-    const uint32_t off = (uint32_t)row * (uint32_t)(ld * L::ES) + (uint32_t)((pos ^ L::f(row)) << 4);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+    if (!EVEN || c0 == 0) {
+      const int ci = c0 + tid, row = ci / L::CPR, pos = ci - row * L::CPR;
+      off = (uint32_t)row * row_bytes + (uint32_t)((pos ^ L::f(row)) << 4);
+    }
+    const uint32_t more = EVEN ? (uint32_t)(c0 / NT * STEP) * row_bytes : 0u;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
                      __builtin_amdgcn_readfirstlane((int)(lds + c0 * 16))),
-                 "v"(off), "s"(rsrc)
+                 "v"(off), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane((int)more))
                  : "memory");
   }
 }

@@ -177,6 +177,12 @@ __device__ __forceinline__ void stage_barrier(bool more, int wid) {
   else tile_barrier<2 * FULL + EXTRA>();
 }
 
+// Operands read from LDS ahead of the matrix instruction that takes them: left to itself the compiler reads each one right before its
+// use and waits out the LDS latency there (dK / dV at T = 4096, hd 128: 850 us).  PIN() keeps the written order.
+template <typename T>
+constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
+#define PIN() __builtin_amdgcn_sched_barrier(0)
+
 // dQ: NW waves of 16 queries; K | V tiles of 32 keys.  S_i^T = K_i Q_i^T and dP^T = V dO^T: keys on the accumulator's rows.
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
@@ -229,39 +235,43 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
     const char *tk = smem, *tv = smem + TILE;
     f32x4 dp[2], s[2][2];
+    // matrix instructions of the step, in order: dP and scores of keys 0 .. 15, of keys 16 .. 31, then the products with K
+    constexpr int NA = 4 * KC, R = AHEAD<T> + 1;
+    Frag<T> ring[R], x[2];
+    auto rows = [&](int u, int i) { return row16<T, HD>(i & 1 ? tk : tv, rk, 16 * u, i / 2); };
+    const bool whole = it * 32 + 32 <= len;
+#pragma unroll
+    for (int i = 0; i < AHEAD<T>; ++i) ring[i] = rows(0, i);
+    PIN();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 2 * KC; ++c) {
-        dp[u] = mma16(row16<T, HD>(tv, rk, 16 * u, c), gf[c], dp[u]);
-        s[c / KC][u] = mma16(row16<T, HD>(tk, rk, 16 * u, c), qf[c], s[c / KC][u]);
+      for (int i = 0; i < NA; ++i) {
+        const int n = i + AHEAD<T>;
+        if (n < NA) ring[n % R] = rows(u, n);
+        else if (u == 0) ring[n % R] = rows(1, n - NA);
+        else ring[n % R] = col16<T, HD>(tk, ck, n - NA);
+        if (i & 1) s[i / 2 / KC][u] = mma16(ring[i % R], qf[i / 2], s[i / 2 / KC][u]);
+        else dp[u] = mma16(ring[i % R], gf[i / 2], dp[u]);
+        PIN();
       }
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float v = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
-          s[m][u][r] = m ? -lam * v : v;
-        }
-    if (it * 32 + 32 > len) {
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (it * 32 + 16 * u + 4 * g + r >= len) s[m][u][r] = 0.f;
+        for (int r = 0; r < 4; ++r) {
+          float v = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
+          if (m) v *= -lam;
+          s[m][u][r] = whole || it * 32 + 16 * u + 4 * g + r < len ? v : 0.f;
+        }
     }
+    frag_from(x[0], s[0][0], s[0][1]);
+    frag_from(x[1], s[1][0], s[1][1]);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      Frag<T> x;
-      frag_from(x, s[m][0], s[m][1]);
-#pragma unroll
-      for (int t = 0; t < CT; ++t) acc[m * CT + t] = mma16(col16<T, HD>(tk, ck, m * CT + t), x, acc[m * CT + t]);
+    for (int t = 0; t < 2 * CT; ++t) {
+      if (t + AHEAD<T> < 2 * CT) ring[(t + AHEAD<T>) % R] = col16<T, HD>(tk, ck, t + AHEAD<T>);
+      acc[t] = mma16(ring[t % R], x[t / CT], acc[t]);
+      PIN();
     }
   }
   if (!qok) return;
@@ -326,13 +336,27 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     const f32x4* ts = reinterpret_cast<const f32x4*>(smem + 2 * TILE + sq);
     f32x4 dp[2], p[2], s[2][2];
     float part = 0.f;
+    // matrix instructions of the step, in order: dP and scores of queries 0 .. 15, of queries 16 .. 31, then the products with dO and Q
+    constexpr int NA = 4 * KC, LEAD = HD == 128 && sizeof(T) == 2 ? 2 : AHEAD<T>, R = LEAD + 1;   // (3 at hd 128: over 256 registers)
+    Frag<T> ring[R], pf, df[2];
+    auto rows = [&](int u, int i) { return row16<T, HD>(i & 1 ? tq : tg, rq, 16 * u, i / 2); };
+    auto cols = [&](int i) { return col16<T, HD>(i & 1 ? tq : tg, cq, i / 2); };
+#pragma unroll
+    for (int i = 0; i < LEAD; ++i) ring[i] = rows(0, i);
+    PIN();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 2 * KC; ++c) {
-        dp[u] = mma16(row16<T, HD>(tg, rq, 16 * u, c), vf[c], dp[u]);
-        s[c / KC][u] = mma16(row16<T, HD>(tq, rq, 16 * u, c), kf[c], s[c / KC][u]);
+      for (int i = 0; i < NA; ++i) {
+        const int n = i + LEAD;
+        Frag<T>&f = ring[(u * NA + i) % R], &ahead = ring[(u * NA + n) % R];
+        if (n < NA) ahead = rows(u, n);
+        else if (u == 0) ahead = rows(1, n - NA);
+        else ahead = cols(n - NA);
+        if (i & 1) s[i / 2 / KC][u] = mma16(f, kf[i / 2], s[i / 2 / KC][u]);
+        else dp[u] = mma16(f, vf[i / 2], dp[u]);
+        PIN();
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -345,14 +369,17 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       }
     }
     dlam += part;
-    Frag<T> pf, df[2];
     frag_from(pf, p[0], p[1]);
     frag_from(df[0], s[0][0], s[0][1]);
     frag_from(df[1], s[1][0], s[1][1]);
 #pragma unroll
-    for (int t = 0; t < 2 * CT; ++t) {
-      dv[t] = mma16(col16<T, HD>(tg, cq, t), pf, dv[t]);
-      dk[t] = mma16(col16<T, HD>(tq, cq, t), df[t / CT], dk[t]);
+    for (int i = 0; i < 4 * CT; ++i) {
+      const int t = i / 2;
+      const Frag<T>& f = ring[(2 * NA + i) % R];
+      if (i + LEAD < 4 * CT) ring[(2 * NA + i + LEAD) % R] = cols(i + LEAD);
+      if (i & 1) dk[t] = mma16(f, df[t / CT], dk[t]);
+      else dv[t] = mma16(f, pf, dv[t]);
+      PIN();
     }
   }
   // a masked key's lane has computed with zeros for its operands and another row's statistics: it gives zeros
