@@ -43,29 +43,30 @@ __device__ __forceinline__ float4 sq4(const float (&v)[8]) {
   return make_float4(v[0] * v[0] + v[4] * v[4], v[1] * v[1] + v[5] * v[5], v[2] * v[2] + v[6] * v[6], v[3] * v[3] + v[7] * v[7]);
 }
 
-// sum over WPR waves that share a row (WPR == 1: one wave; else the whole workgroup is one row's)
-template <int WPR>
+// sum over the W waves of a workgroup (one row)
+template <int W>
 __device__ __forceinline__ float row_sum(float v, float* red) {
   v = wave_sum(v);
-  if constexpr (WPR > 1) {
+  if constexpr (W > 1) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int i = 1; i < WPR; ++i) v += red[i];
+    for (int i = 1; i < W; ++i) v += red[i];
   }
   return v;
 }
 
-// Vector path: 8 | d, 16-byte aligned rows, d <= 64 * WPR * 8 * NC.  A lane owns NC groups of 8 columns (one Philox block each).
+// Vector path: 8 | d, 16-byte aligned rows, d <= 512 W NC.  One workgroup of W waves per row; a lane owns NC groups of 8 columns (one
+// Philox block each).  W = ceil(d / 512), so that few lanes idle and a lane holds little: the waves in flight hide the row's one
+// round trip (a wave per row, 3 - 4 groups per lane: 13312 x 2048 training 71 -> 60 us, 8-bit 8320 x 1536 30.4 -> 28.3 us).
 // H: type of h and of y (unless MX); X: type of the stream.
-template <typename H, typename X, bool MX, int NC, int WPR>
-__global__ __launch_bounds__(256) void add_rmsnorm_kernel(Fwd a) {
-  __shared__ float red[4];
-  constexpr int LANES = 64 * WPR;
-  const int lane = threadIdx.x & (LANES - 1);
-  const int64_t row = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (4 / WPR) + (threadIdx.x / LANES);
-  if (row >= a.rows) return;                                   // wave-uniform (WPR == 1) or never taken (WPR == 4)
+template <typename H, typename X, bool MX, int NC, int W>
+__global__ __launch_bounds__(64 * W) void add_rmsnorm_kernel(Fwd a) {
+  __shared__ float red[W];
+  constexpr int LANES = 64 * W;
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
   const int n8 = (int)(a.d >> 3);
   const X* rr = (const X*)a.resid + row * a.ldr;
   float x[NC][8];
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_kernel(Fwd a) {
     const float4 q = sq4(x[i]);
     s += (q.x + q.y) + (q.z + q.w);
   }
-  const float rho = 1.0f / sqrtf(row_sum<WPR>(s, red) * a.inv_d + a.eps);
+  const float rho = 1.0f / sqrtf(row_sum<W>(s, red) * a.inv_d + a.eps);
   if (a.rho && lane == 0) a.rho[row] = rho;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
@@ -195,21 +196,14 @@ int launch_fwd(const Fwd& a, bool vec, hipStream_t s) {
     hipLaunchKernelGGL((add_rmsnorm_any_kernel<H, X, MX>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
     return gpt_launch_status("gpt_add_rmsnorm");
   }
-  // a wave per row, or a workgroup per row: where waves alone would leave CUs empty, and where a row does not fit a wave's registers
-  const bool wide = a.d > 2048 || a.rows < 2048;
   GPT_REQUIRE(a.rows < (1ll << 24), "gpt_add_rmsnorm: too many rows (%lld)", (long long)a.rows);
-#define RN(NC, WPR) \
-  hipLaunchKernelGGL((add_rmsnorm_kernel<H, X, MX, NC, WPR>), dim3((unsigned)((a.rows + 4 / WPR - 1) / (4 / WPR))), dim3(256), 0, s, a)
-  if (wide) {
-    if (a.d <= 2048) RN(1, 4);
-    else if (a.d <= 4096) RN(2, 4);
-    else RN(4, 4);
-  } else {
-    if (a.d <= 512) RN(1, 1);
-    else if (a.d <= 1024) RN(2, 1);
-    else if (a.d <= 1536) RN(3, 1);
-    else RN(4, 1);
-  }
+#define RN(NC, W) hipLaunchKernelGGL((add_rmsnorm_kernel<H, X, MX, NC, W>), dim3((unsigned)a.rows), dim3(64 * W), 0, s, a)
+  if (a.d <= 512) RN(1, 1);
+  else if (a.d <= 1024) RN(1, 2);
+  else if (a.d <= 1536) RN(1, 3);
+  else if (a.d <= 2048) RN(1, 4);
+  else if (a.d <= 4096) RN(2, 4);
+  else RN(4, 4);
 #undef RN
   return gpt_launch_status("gpt_add_rmsnorm");
 }
@@ -225,14 +219,14 @@ struct Bwd {
   DropoutRng rng;
 };
 
-constexpr int BWD_BLOCKS = 512;  // workgroups at most: rows are dealt out round robin, each keeps its columns' dw sums in registers
+constexpr int BWD_BLOCKS = 768;  // workgroups at most: rows are dealt out round robin, each keeps its columns' dw sums in registers
 
-// Vector path, one wave per row (WPR == 1) or one workgroup per row (WPR == 4)
-template <typename H, typename X, int NC, int WPR>
-__global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(Bwd a) {
-  __shared__ __attribute__((aligned(16))) float sums[WPR == 1 ? 4 * 512 * NC : 4];
-  constexpr int LANES = 64 * WPR, RPB = 4 / WPR;
-  const int lane = threadIdx.x & (LANES - 1), sub = threadIdx.x / LANES;
+// Vector path, one workgroup of W waves per row at a time
+template <typename H, typename X, int NC, int W>
+__global__ __launch_bounds__(64 * W) void add_rmsnorm_bwd_kernel(Bwd a) {
+  __shared__ float red[W];
+  constexpr int LANES = 64 * W;
+  const int lane = threadIdx.x;
   const int n8 = (int)(a.d >> 3);
   const uint64_t off = a.rng.thr ? dropout_offset(a.rng) : 0;
   float dw[NC][8];
@@ -240,8 +234,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(Bwd a) {
   for (int i = 0; i < NC; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
-  // WPR == 4: the bound is uniform over the workgroup, so its barriers are met by all waves
-  for (int64_t row = (int64_t)blockIdx.x * RPB + sub; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float x[NC][8], t[NC][8], g[NC][8];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -268,8 +261,8 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(Bwd a) {
         }
       }
     }
-    if constexpr (WPR > 1) __syncthreads();                       // the previous row's sums have been read
-    const float k = rho * rho * rho * (row_sum<WPR>(s, sums) * a.inv_d);
+    if constexpr (W > 1) __syncthreads();                         // the previous row's sums have been read
+    const float k = rho * rho * rho * (row_sum<W>(s, red) * a.inv_d);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = lane + LANES * i;
@@ -291,26 +284,10 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_kernel(Bwd a) {
   }
   if (!a.part) return;
   float* out = a.part + (int64_t)blockIdx.x * a.d;
-  if constexpr (WPR == 1) {
-    // the four waves' sums through LDS, added in wave order
 #pragma unroll
-    for (int i = 0; i < NC; ++i) store8(&sums[sub * 512 * NC + (lane + 64 * i) * 8], dw[i]);
-    __syncthreads();
-    for (int c = threadIdx.x * 4; c < (int)a.d; c += 1024) {
-      float4 v = *reinterpret_cast<const float4*>(&sums[c]);
-#pragma unroll
-      for (int q = 1; q < 4; ++q) {
-        const float4 u = *reinterpret_cast<const float4*>(&sums[q * 512 * NC + c]);
-        v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
-      }
-      *reinterpret_cast<float4*>(out + c) = v;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = lane + LANES * i;
-      if (c < n8) store8(out + c * 8, dw[i]);
-    }
+  for (int i = 0; i < NC; ++i) {
+    const int c = lane + LANES * i;
+    if (c < n8) store8(out + c * 8, dw[i]);
   }
 }
 
@@ -366,27 +343,17 @@ __global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* __restric
   }
 }
 
-int bwd_blocks(int64_t rows, bool wave_rows) {
-  const int64_t want = wave_rows ? (rows + 3) / 4 : rows;
-  return (int)(want < BWD_BLOCKS ? want : BWD_BLOCKS);
-}
-
 template <typename H, typename X>
 int launch_bwd(const Bwd& a, bool vec, float* dweight, hipStream_t s) {
-  const bool any = !vec || a.d > 8192, wave_rows = !any && a.d <= 2048 && a.rows >= 2048;
-  const int nb = bwd_blocks(a.rows, wave_rows);
-#define RB(NC, WPR) hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<H, X, NC, WPR>), dim3(nb), dim3(256), 0, s, a)
-  if (any) hipLaunchKernelGGL((add_rmsnorm_bwd_any_kernel<H, X>), dim3(nb), dim3(256), 0, s, a);
-  else if (wave_rows) {
-    if (a.d <= 512) RB(1, 1);
-    else if (a.d <= 1024) RB(2, 1);
-    else if (a.d <= 1536) RB(3, 1);
-    else RB(4, 1);
-  } else {
-    if (a.d <= 2048) RB(1, 4);
-    else if (a.d <= 4096) RB(2, 4);
-    else RB(4, 4);
-  }
+  const int nb = (int)(a.rows < BWD_BLOCKS ? a.rows : BWD_BLOCKS);
+#define RB(NC, W) hipLaunchKernelGGL((add_rmsnorm_bwd_kernel<H, X, NC, W>), dim3(nb), dim3(64 * W), 0, s, a)
+  if (!vec || a.d > 8192) hipLaunchKernelGGL((add_rmsnorm_bwd_any_kernel<H, X>), dim3(nb), dim3(256), 0, s, a);
+  else if (a.d <= 512) RB(1, 1);
+  else if (a.d <= 1024) RB(1, 2);
+  else if (a.d <= 1536) RB(1, 3);
+  else if (a.d <= 2048) RB(1, 4);
+  else if (a.d <= 4096) RB(2, 4);
+  else RB(4, 4);
 #undef RB
   if (int st = gpt_launch_status("gpt_add_rmsnorm_bwd")) return st;
   if (dweight) {
