@@ -156,72 +156,78 @@ __global__ __launch_bounds__(64) void short_fwd_kernel(Args a) {
   store_tile<T, HD>((T*)a.out + (int64_t)b * a.bso + h * 2 * HD, a.ldo, a.Tq, tq, lane);
 }
 
-// the [query][key] matrices that go through LDS: pitch in bytes (bf16: rows 18 banks apart, conflict-free for the 8-byte writes of
-// 32 rows and for the 4-row transposing reads)
+// A [query][key] matrix on its way through LDS: pitch in bytes (bf16: rows 18 banks apart, conflict-free for the 8-byte writes of 32
+// rows and for the 4-row transposing reads)
 template <typename T>
 constexpr int P_PITCH = sizeof(T) == 2 ? 72 : 144;
-template <typename T>
-constexpr int P_BYTES = 32 * P_PITCH<T>;
 
 template <typename T>
 __device__ __forceinline__ void put_matrix(char* m, const f32x16& x, int r, int hh) {
 #pragma unroll
   for (int g = 0; g < 4; ++g) store4((T*)(m + r * P_PITCH<T>) + 8 * g + 4 * hh, f32x4{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]});
 }
-// as an operand that contracts over its rows (queries, ascending), keys on the lanes
+// n rows of it as an operand that contracts over the rows (queries, ascending), keys on the lanes
 template <typename T>
-__device__ __forceinline__ void get_matrix(Operand& o, const char* m, int lane) {
+__device__ __forceinline__ void get_matrix(Operand& o, const char* m, int n, int lane, const char* zero) {
   if constexpr (sizeof(T) == 2) {
     const int gq = lane >> 4, tq = (lane & 15) >> 2, tp = lane & 3;
-    const char* base = m + (8 * (gq >> 1) + tq) * P_PITCH<T> + (16 * (gq & 1) + 4 * tp) * 2;
+    const int col = (16 * (gq & 1) + 4 * tp) * 2;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(base + 16 * s * P_PITCH<T>));
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(base + (16 * s + 4) * P_PITCH<T>));
+      const int r0 = 16 * s + 8 * (gq >> 1) + tq, r1 = r0 + 4;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(r0 < n ? m + r0 * P_PITCH<T> + col : zero));
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(r1 < n ? m + r1 * P_PITCH<T> + col : zero));
       o.p[s] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 16; ++e) o.f[e] = reinterpret_cast<const float*>(m + (2 * e + (lane >> 5)) * P_PITCH<T>)[lane & 31];
+    for (int e = 0; e < 16; ++e) {
+      const int q = 2 * e + (lane >> 5);
+      o.f[e] = *reinterpret_cast<const float*>(q < n ? m + q * P_PITCH<T> + (lane & 31) * 4 : zero);
+    }
   }
-}
-
-// V's tile, large enough for the three matrices that follow it there
-template <typename T, int HD>
-__host__ __device__ constexpr int v_bytes(int Tk) {
-  return Tk * Tile<T, HD>::PITCH > 3 * P_BYTES<T> ? Tk * Tile<T, HD>::PITCH : 3 * P_BYTES<T>;
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(64) void short_bwd_kernel(Args a) {
   using L = Tile<T, HD>;
-  constexpr int NT = 2 * HD / 32;
+  constexpr int NT = 2 * HD / 32, HALF = NT / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x, r = lane & 31, hh = lane >> 5;
   const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, len = valid_keys(a, b);
-  char *tq = smem, *tg = tq + a.Tq * L::PITCH, *tk = tg + a.Tq * L::PITCH, *tv = tk + a.Tk * L::PITCH;
-  char* zero = tv + v_bytes<T, HD>(a.Tk);
+  const int rows = a.Tq > a.Tk ? a.Tq : a.Tk;
+  char *tq = smem, *tg = tq + rows * L::PITCH, *tk = tg + rows * L::PITCH, *tm = tk + rows * L::PITCH, *zero = tm + a.Tq * P_PITCH<T>;
   if (lane < 4) reinterpret_cast<uint32_t*>(zero)[lane] = 0u;
   load_tile<T, HD>((const T*)a.q + (int64_t)b * a.bsq + h * 2 * HD, a.ldq, a.Tq, a.Tq, tq, lane);
   load_tile<T, HD>((const T*)a.k + (int64_t)b * a.bsk + h * 2 * HD, a.ldk, a.Tk, len, tk, lane);
-  load_tile<T, HD>((const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD, a.ldv, a.Tk, len, tv, lane);
   load_tile<T, HD>((const T*)a.dout + (int64_t)b * a.bsdo + h * 2 * HD, a.lddo, a.Tq, a.Tq, tg, lane);
+  // V is only used by rows, once: straight to registers, no LDS (5 instead of 4 waves per CU at 26 tokens, hd 96)
+  const bool qok = r < a.Tq, kok = r < a.Tk, vok = r < len;
+  u32x4 vf[L::CPR / 2];
+  {
+    const u32x4* vr = reinterpret_cast<const u32x4*>((const T*)a.v + (int64_t)b * a.bsv + (int64_t)(vok ? r : 0) * a.ldv + h * 2 * HD);
+#pragma unroll
+    for (int c = 0; c < L::CPR / 2; ++c) {
+      vf[c] = u32x4{0u, 0u, 0u, 0u};
+      if (vok) vf[c] = vr[2 * c + hh];
+    }
+  }
+  const float lam = a.lam[h];
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  const bool qok = r < a.Tq, kok = r < a.Tk;
-  f32x16 s[2];
+  f32x16 s[2], dp = zero16();
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     s[m] = rows_product<T, HD>(tk, kok, tq, qok, r, hh, m * L::CM, L::CM, zero);
     softmax32(s[m], len, hh, a.c2);
   }
-  const f32x16 dp = rows_product<T, HD>(tv, kok, tg, qok, r, hh, 0, L::CPR, zero);
-  const float lam = a.lam[h];
+#pragma unroll
+  for (int c = 0; c < L::CPR / 2; ++c) dp = mma_chunk<T>(vf[c], *reinterpret_cast<const u32x4*>(qok ? tg + L::at(r, 2 * c + hh) : zero), dp);
   float d[2] = {0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) d[m] += row_of(e, hh) < len ? s[m][e] * dp[e] : 0.f;
-    d[m] += __shfl_xor(d[m], 32, 64);
+    d[m] = col_sum(d[m]);
   }
   const float dl = wave_sum(qok && hh == 0 ? d[1] : 0.f);
   if (lane == 0) a.dlam_part[(int64_t)h * a.B + b] = dl;
@@ -233,46 +239,41 @@ __global__ __launch_bounds__(64) void short_bwd_kernel(Args a) {
     s[0][e] = in ? s[0][e] * (dp[e] - d[0]) : 0.f;
     s[1][e] = in ? -lam * (s[1][e] * (dp[e] - d[1])) : 0.f;
   }
-  lds_done();                                               // V has been read: its tile takes P, dS_1, dS_2
-  put_matrix<T>(tv, p, r, hh);
-  put_matrix<T>(tv + P_BYTES<T>, s[0], r, hh);
-  put_matrix<T>(tv + 2 * P_BYTES<T>, s[1], r, hh);
-  Operand x[2];
-  f32x16 acc[NT];
-  // dQ_i^T = K_i^T dS_i^T, staged in K's tile once K has been read
+  // dS_i^T is dQ's operand as it stands; P, dS_1 and dS_2 go through the one matrix buffer in turn
+  Operand x, xp, xs[2];
+  if (qok) put_matrix<T>(tm, p, r, hh);
+  lds_done();
+  get_matrix<T>(xp, tm, a.Tq, lane, zero);
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    operand_from<T>(x[m], s[m]);
-#pragma unroll
-    for (int t = 0; t < NT / 2; ++t) acc[m * NT / 2 + t] = columns_product<T, HD, 0>(tk, a.Tk, m * NT / 2 + t, x[m], lane, zero);
+    lds_done();
+    if (qok) put_matrix<T>(tm, s[m], r, hh);
+    lds_done();
+    get_matrix<T>(xs[m], tm, a.Tq, lane, zero);
   }
-  lds_done();
-  // (K's tile has Tk rows, Q's and dO's Tq: an output goes to a tile of its own row count)
-  Operand xp;
-  get_matrix<T>(x[0], tv + P_BYTES<T>, lane);
-  get_matrix<T>(x[1], tv + 2 * P_BYTES<T>, lane);
-  get_matrix<T>(xp, tv, lane);
-  f32x16 dk[NT];
+  // each output leaves through the tile of the operand that its products have just read (all tiles have max(Tq, Tk) rows)
+  f32x16 acc[NT];
+  auto put = [&](char* tile, T* dst, int64_t ld, int n, float scale) {
+    lds_done();
 #pragma unroll
-  for (int t = 0; t < NT; ++t) dk[t] = columns_product<T, HD, 1>(tq, a.Tq, t, x[t / (NT / 2)], lane, zero);
-  lds_done();
+    for (int t = 0; t < NT; ++t)
+      if (r < n) stage<T, HD>(tile, r, hh, t, acc[t], scale);
+    lds_done();
+    store_tile<T, HD>(dst, ld, n, tile, lane);
+  };
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    if (qok) stage<T, HD>(tq, r, hh, t, acc[t], a.scale);
-    if (kok) stage<T, HD>(tk, r, hh, t, dk[t], a.scale);
+  for (int m = 0; m < 2; ++m) {
+    operand_from<T>(x, s[m]);
+#pragma unroll
+    for (int t = m * HALF; t < (m + 1) * HALF; ++t) acc[t] = columns_product<T, HD, 0>(tk, a.Tk, t, x, lane, zero);       // dQ_m^T = K_m^T dS_m^T
   }
-  lds_done();
-  store_tile<T, HD>((T*)a.dq + (int64_t)b * a.bsdq + h * 2 * HD, a.lddq, a.Tq, tq, lane);
-  store_tile<T, HD>((T*)a.dk + (int64_t)b * a.bsdk + h * 2 * HD, a.lddk, a.Tk, tk, lane);
-  // dV^T = dO^T P
+  put(tk, (T*)a.dq + (int64_t)b * a.bsdq + h * 2 * HD, a.lddq, a.Tq, a.scale);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = columns_product<T, HD, 1>(tg, a.Tq, t, xp, lane, zero);
-  lds_done();
+  for (int t = 0; t < NT; ++t) acc[t] = columns_product<T, HD, 1>(tq, a.Tq, t, xs[t / HALF], lane, zero);                 // dK_m^T = Q_m^T dS_m
+  put(tq, (T*)a.dk + (int64_t)b * a.bsdk + h * 2 * HD, a.lddk, a.Tk, a.scale);
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-    if (kok) stage<T, HD>(tk, r, hh, t, acc[t], 1.f);
-  lds_done();
-  store_tile<T, HD>((T*)a.dv + (int64_t)b * a.bsdv + h * 2 * HD, a.lddv, a.Tk, tk, lane);
+  for (int t = 0; t < NT; ++t) acc[t] = columns_product<T, HD, 1>(tg, a.Tq, t, xp, lane, zero);                           // dV^T = dO^T P
+  put(tg, (T*)a.dv + (int64_t)b * a.bsdv + h * 2 * HD, a.lddv, a.Tk, 1.f);
 }
 
 template <typename T, int HD>
@@ -288,7 +289,7 @@ int go(const Args& a, bool backward, hipStream_t s) {
   }
   const char* who = "gpt_diff_attention_bwd";
   if (int st = grant_lds(short_bwd_kernel<T, HD>, bwd_once, who)) return st;
-  const int lds = (2 * a.Tq + a.Tk) * L::PITCH + v_bytes<T, HD>(a.Tk) + 16;
+  const int lds = 3 * (a.Tq > a.Tk ? a.Tq : a.Tk) * L::PITCH + a.Tq * P_PITCH<T> + 16;
   hipLaunchKernelGGL((short_bwd_kernel<T, HD>), grid, dim3(64), lds, s, a);
   return gpt_launch_status(who);
 }
