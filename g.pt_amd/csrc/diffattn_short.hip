@@ -124,33 +124,46 @@ __device__ __forceinline__ void softmax32(f32x16& s, int len, int hh, float c2) 
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(64) void short_fwd_kernel(Args a) {
+__global__ __launch_bounds__(64, sizeof(T) == 2 ? 3 : 1) void short_fwd_kernel(Args a) {
   using L = Tile<T, HD>;
+  constexpr int NT = 2 * HD / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x, r = lane & 31, hh = lane >> 5;
   const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, len = valid_keys(a, b);
-  char *tq = smem, *tk = tq + a.Tq * L::PITCH, *tv = tk + a.Tk * L::PITCH, *zero = tv + a.Tk * L::PITCH;
+  char *tq = smem, *tv = tq + a.Tq * L::PITCH, *zero = tv + a.Tk * L::PITCH;
   if (lane < 4) reinterpret_cast<uint32_t*>(zero)[lane] = 0u;
   load_tile<T, HD>((const T*)a.q + (int64_t)b * a.bsq + h * 2 * HD, a.ldq, a.Tq, a.Tq, tq, lane);
-  load_tile<T, HD>((const T*)a.k + (int64_t)b * a.bsk + h * 2 * HD, a.ldk, a.Tk, len, tk, lane);
-  load_tile<T, HD>((const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD, a.ldv, a.Tk, len, tv, lane);
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-  f32x16 s[2];
+  // K is only used by rows, once: straight to registers
+  const bool kok = r < len, qok = r < a.Tq;
+  u32x4 kf[L::CPR / 2];
+  {
+    const u32x4* kr = reinterpret_cast<const u32x4*>((const T*)a.k + (int64_t)b * a.bsk + (int64_t)(kok ? r : 0) * a.ldk + h * 2 * HD);
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    s[m] = rows_product<T, HD>(tk, r < a.Tk, tq, r < a.Tq, r, hh, m * L::CM, L::CM, zero);
-    softmax32(s[m], len, hh, a.c2);
+    for (int c = 0; c < L::CPR / 2; ++c) {
+      kf[c] = u32x4{0u, 0u, 0u, 0u};
+      if (kok) kf[c] = kr[2 * c + hh];
+    }
   }
+  load_tile<T, HD>((const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD, a.ldv, a.Tk, len, tv, lane);
   const float lam = a.lam[h];
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+  for (int c = 0; c < L::CPR / 2; ++c) {
+    const int m = c >= L::CM / 2;
+    s[m] = mma_chunk<T>(kf[c], *reinterpret_cast<const u32x4*>(qok ? tq + L::at(r, 2 * c + hh) : zero), s[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < 2; ++m) softmax32(s[m], len, hh, a.c2);
   Operand p;
 #pragma unroll
   for (int e = 0; e < 16; ++e) s[0][e] -= lam * s[1][e];
   operand_from<T>(p, s[0]);                                 // bf16: the difference of the maps is rounded, once
   lds_done();                                               // Q has been read: its tile takes the output
 #pragma unroll
-  for (int t = 0; t < 2 * HD / 32; ++t) {
+  for (int t = 0; t < NT; ++t) {
     const f32x16 o = columns_product<T, HD, 0>(tv, a.Tk, t, p, lane, zero);
-    if (r < a.Tq) stage<T, HD>(tq, r, hh, t, o, 1.f);
+    if (qok) stage<T, HD>(tq, r, hh, t, o, 1.f);
   }
   lds_done();
   store_tile<T, HD>((T*)a.out + (int64_t)b * a.bso + h * 2 * HD, a.ldo, a.Tq, tq, lane);
@@ -189,7 +202,7 @@ __device__ __forceinline__ void get_matrix(Operand& o, const char* m, int n, int
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(64) void short_bwd_kernel(Args a) {
+__global__ __launch_bounds__(64, sizeof(T) == 2 && HD < 128 ? 2 : 1) void short_bwd_kernel(Args a) {
   using L = Tile<T, HD>;
   constexpr int NT = 2 * HD / 32, HALF = NT / 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -284,7 +297,7 @@ int go(const Args& a, bool backward, hipStream_t s) {
   if (!backward) {
     const char* who = "gpt_diff_attention";
     if (int st = grant_lds(short_fwd_kernel<T, HD>, fwd_once, who)) return st;
-    hipLaunchKernelGGL((short_fwd_kernel<T, HD>), grid, dim3(64), (a.Tq + 2 * a.Tk) * L::PITCH + 16, s, a);
+    hipLaunchKernelGGL((short_fwd_kernel<T, HD>), grid, dim3(64), (a.Tq + a.Tk) * L::PITCH + 16, s, a);
     return gpt_launch_status(who);
   }
   const char* who = "gpt_diff_attention_bwd";
