@@ -164,19 +164,9 @@ __global__ __launch_bounds__(256) void stats_kernel(Args a, f32x4* stats) {
   }
 }
 
-// stages of the tile ring: three where the LDS allows (the tile after next is in flight while one is used)
+// stages of the tile ring: the tile in use, the next one in flight and, where the halves of a workgroup run a part apart, the one before
 template <typename T, int NW>
 constexpr int STAGES = sizeof(T) == 2 && NW == 8 ? 3 : 2;
-// The next of NS stages is here.  With three, what was issued after it - two tiles of 32 rows and EXTRA instructions of this wave -
-// may stay in flight.  (The last chunks of a tile may be fewer than the threads: then only the first waves have issued one more.)
-template <typename T, int HD, int NW, int EXTRA>
-__device__ __forceinline__ void stage_barrier(bool more, int wid) {
-  constexpr int CHUNKS = 32 * Tile<T, HD>::CPR, FULL = CHUNKS / (NW * 64), REM = CHUNKS % (NW * 64);
-  if (STAGES<T, NW> < 3 || !more) tile_barrier<0>();
-  else if (REM != 0 && wid * 64 < REM) tile_barrier<2 * (FULL + 1) + EXTRA>();
-  else tile_barrier<2 * FULL + EXTRA>();
-}
-
 // Operands read from LDS ahead of the matrix instruction that takes them: left to itself the compiler reads each one right before its
 // use and waits out the LDS latency there (dK / dV at T = 4096, hd 128: 850 us).  PIN() keeps the written order.
 template <typename T>
@@ -221,25 +211,18 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     dma_tile<T, HD, 32, NT>(kb + (int64_t)it * 32 * a.ldk, a.ldk, len - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(vb + (int64_t)it * 32 * a.ldv, a.ldv, len - it * 32, dst + TILE, tid, wid);
   };
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < n) fetch(i, i * STAGE);
-  int now = 0, next = (NS - 1) * STAGE;                                      // stages in use and to be filled
-  for (int it = 0; it < n; ++it) {
-    stage_barrier<T, HD, NW, 0>(it + 1 < n, wid);
-    if (it + NS - 1 < n) fetch(it + NS - 1, next);                           // into the buffer that was read before the barrier
-    // the lane's places in this stage, opaque to the compiler: it would keep every variant of them in a register over the loop
-    int rk = rb + now, ck = cb + now;
-    asm volatile("" : "+v"(rk), "+v"(ck));
-    next = now;
-    now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
-    const char *tk = smem, *tv = smem + TILE;
-    f32x4 dp[2], s[2][2];
-    // matrix instructions of the step, in order: dP and scores of keys 0 .. 15, of keys 16 .. 31, then the products with K
-    constexpr int NA = 4 * KC, R = AHEAD<T> + 1;
-    Frag<T> ring[R], x[2];
-    auto rows = [&](int u, int i) { return row16<T, HD>(i & 1 ? tk : tv, rk, 16 * u, i / 2); };
-    const bool whole = it * 32 + 32 <= len;
+  // The step's three parts: scores and dP (matrix), dS (vector), products with K (matrix).  All waves meet at one barrier per tile, and
+  // the two waves of a SIMD would do the same part at the same time: the workgroup's second half runs a part behind, its products with
+  // K taken from the tile before while the first half computes scores.
+  constexpr int NA = 4 * KC, R = AHEAD<T> + 1;
+  const bool late = NS == 3 && wid >= NW / 2;
+  f32x4 dp[2], s[2][2];
+  Frag<T> ring[R], x[2];
+  auto scores = [&](int at, int it) {
+    // the lane's place in this stage, opaque to the compiler: it would keep every variant of it in a register over the loop
+    int rk = rb + at;
+    asm volatile("" : "+v"(rk));
+    auto rows = [&](int u, int i) { return row16<T, HD>(smem + (i & 1 ? 0 : TILE), rk, 16 * u, i / 2); };
 #pragma unroll
     for (int i = 0; i < AHEAD<T>; ++i) ring[i] = rows(0, i);
     PIN();
@@ -248,36 +231,62 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
       dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NA; ++i) {
-        const int n = i + AHEAD<T>;
-        if (n < NA) ring[n % R] = rows(u, n);
-        else if (u == 0) ring[n % R] = rows(1, n - NA);
-        else ring[n % R] = col16<T, HD>(tk, ck, n - NA);
-        if (i & 1) s[i / 2 / KC][u] = mma16(ring[i % R], qf[i / 2], s[i / 2 / KC][u]);
-        else dp[u] = mma16(ring[i % R], gf[i / 2], dp[u]);
+        const int n = u * NA + i + AHEAD<T>;
+        if (n < 2 * NA) ring[n % R] = rows(n / NA, n % NA);
+        const Frag<T>& f = ring[(u * NA + i) % R];
+        if (i & 1) s[i / 2 / KC][u] = mma16(f, qf[i / 2], s[i / 2 / KC][u]);
+        else dp[u] = mma16(f, gf[i / 2], dp[u]);
         PIN();
       }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[m][u][r] = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
+    if (it * 32 + 32 > len) {
 #pragma unroll
       for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
-          if (m) v *= -lam;
-          s[m][u][r] = whole || it * 32 + 16 * u + 4 * g + r < len ? v : 0.f;
-        }
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (it * 32 + 16 * u + 4 * g + r >= len) s[m][u][r] = 0.f;
     }
     frag_from(x[0], s[0][0], s[0][1]);
     frag_from(x[1], s[1][0], s[1][1]);
+  };
+  auto products = [&](int at) {
+    int ck = cb + at;
+    asm volatile("" : "+v"(ck));
+#pragma unroll
+    for (int t = 0; t < AHEAD<T>; ++t) ring[t] = col16<T, HD>(smem, ck, t);
+    PIN();
 #pragma unroll
     for (int t = 0; t < 2 * CT; ++t) {
-      if (t + AHEAD<T> < 2 * CT) ring[(t + AHEAD<T>) % R] = col16<T, HD>(tk, ck, t + AHEAD<T>);
+      if (t + AHEAD<T> < 2 * CT) ring[(t + AHEAD<T>) % R] = col16<T, HD>(smem, ck, t + AHEAD<T>);
       acc[t] = mma16(ring[t % R], x[t / CT], acc[t]);
       PIN();
     }
+  };
+  int before = 0, now = 0;                                                  // stages of the previous tile and of this one
+  if (n > 0) fetch(0, 0);
+  for (int it = 0; it < n; ++it) {
+    tile_barrier<0>();
+    const int next = now + STAGE == NS * STAGE ? 0 : now + STAGE;
+    if (it + 1 < n) fetch(it + 1, next);                                     // the buffer of two tiles (NS == 2: one tile) ago
+    if (late && it > 0) products(before);
+    scores(now, it);
+    if (!late) products(now);
+    before = now;
+    now = next;
   }
+  if (late && n > 0) products(before);
   if (!qok) return;
   T* dq = (T*)a.dq + (int64_t)b * a.bsdq + (int64_t)qi * a.lddq + h * 2 * HD + 4 * g;
 #pragma unroll
-  for (int t = 0; t < 2 * CT; ++t) store4(dq + t * 16, acc[t] * a.scale);
+  for (int t = 0; t < 2 * CT; ++t) store4(dq + t * 16, acc[t] * (t < CT ? a.scale : -lam * a.scale));   // -lam of dS_2: here, once
 }
 
 // dK, dV and the tile's share of sum P_2 dP: NW waves of 16 keys; Q | dO | statistics tiles of 32 queries.  S_i = Q_i K_i^T and
@@ -319,28 +328,18 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     char* dst = smem + at;
     dma_tile<T, HD, 32, NT>(qb + (int64_t)it * 32 * a.ldq, a.ldq, a.Tq - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(gb + (int64_t)it * 32 * a.lddo, a.lddo, a.Tq - it * 32, dst + TILE, tid, wid);
-    dma_bytes(sb + it * 32, (a.Tq - it * 32) * 16, dst + 2 * TILE, lane);    // every wave the same 512 bytes: one count for all
+    if (wid == 0) dma_bytes(sb + it * 32, (a.Tq - it * 32) * 16, dst + 2 * TILE, lane);
   };
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < n) fetch(i, i * STAGE);
-  int now = 0, next = (NS - 1) * STAGE;
-  for (int it = 0; it < n; ++it) {
-    stage_barrier<T, HD, NW, 1>(it + 1 < n, wid);
-    if (it + NS - 1 < n) fetch(it + NS - 1, next);
-    int rq = rb + now, cq = cb + now, sq = 64 * g + now;                     // as in dq_kernel
-    asm volatile("" : "+v"(rq), "+v"(cq), "+v"(sq));
-    next = now;
-    now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
-    const char *tq = smem, *tg = smem + TILE;
+  constexpr int NA = 4 * KC, LEAD = HD == 128 && sizeof(T) == 2 ? 2 : AHEAD<T>, R = LEAD + 1;   // (3 at hd 128: over 256 registers)
+  const bool late = NS == 3 && wid >= NW / 2;                               // as in dq_kernel
+  f32x4 dp[2], p[2], s[2][2];
+  Frag<T> ring[R], pf, df[2];
+  auto scores = [&](int at) {
+    int rq = rb + at, sq = 64 * g + at;
+    asm volatile("" : "+v"(rq), "+v"(sq));
     const f32x4* ts = reinterpret_cast<const f32x4*>(smem + 2 * TILE + sq);
-    f32x4 dp[2], p[2], s[2][2];
+    auto rows = [&](int u, int i) { return row16<T, HD>(smem + (i & 1 ? 0 : TILE), rq, 16 * u, i / 2); };
     float part = 0.f;
-    // matrix instructions of the step, in order: dP and scores of queries 0 .. 15, of queries 16 .. 31, then the products with dO and Q
-    constexpr int NA = 4 * KC, LEAD = HD == 128 && sizeof(T) == 2 ? 2 : AHEAD<T>, R = LEAD + 1;   // (3 at hd 128: over 256 registers)
-    Frag<T> ring[R], pf, df[2];
-    auto rows = [&](int u, int i) { return row16<T, HD>(i & 1 ? tq : tg, rq, 16 * u, i / 2); };
-    auto cols = [&](int i) { return col16<T, HD>(i & 1 ? tq : tg, cq, i / 2); };
 #pragma unroll
     for (int i = 0; i < LEAD; ++i) ring[i] = rows(0, i);
     PIN();
@@ -349,15 +348,16 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       dp[u] = s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NA; ++i) {
-        const int n = i + LEAD;
-        Frag<T>&f = ring[(u * NA + i) % R], &ahead = ring[(u * NA + n) % R];
-        if (n < NA) ahead = rows(u, n);
-        else if (u == 0) ahead = rows(1, n - NA);
-        else ahead = cols(n - NA);
+        const int n = u * NA + i + LEAD;
+        if (n < 2 * NA) ring[n % R] = rows(n / NA, n % NA);
+        const Frag<T>& f = ring[(u * NA + i) % R];
         if (i & 1) s[i / 2 / KC][u] = mma16(f, kf[i / 2], s[i / 2 / KC][u]);
         else dp[u] = mma16(f, vf[i / 2], dp[u]);
         PIN();
       }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x4 st = ts[16 * u + r];
@@ -365,23 +365,42 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         p[u][r] = p0 - lam * p1;
         part += p1 * dp[u][r];
         s[0][u][r] = p0 * (dp[u][r] - st[2]);
-        s[1][u][r] = -lam * (p1 * (dp[u][r] - st[3]));
+        s[1][u][r] = p1 * (dp[u][r] - st[3]);                                // -lam: at the end, once
       }
-    }
     dlam += part;
     frag_from(pf, p[0], p[1]);
     frag_from(df[0], s[0][0], s[0][1]);
     frag_from(df[1], s[1][0], s[1][1]);
+  };
+  auto products = [&](int at) {
+    int cq = cb + at;
+    asm volatile("" : "+v"(cq));
+    auto cols = [&](int i) { return col16<T, HD>(smem + (i & 1 ? 0 : TILE), cq, i / 2); };
+#pragma unroll
+    for (int i = 0; i < LEAD; ++i) ring[i] = cols(i);
+    PIN();
 #pragma unroll
     for (int i = 0; i < 4 * CT; ++i) {
       const int t = i / 2;
-      const Frag<T>& f = ring[(2 * NA + i) % R];
-      if (i + LEAD < 4 * CT) ring[(2 * NA + i + LEAD) % R] = cols(i + LEAD);
-      if (i & 1) dk[t] = mma16(f, df[t / CT], dk[t]);
-      else dv[t] = mma16(f, pf, dv[t]);
+      if (i + LEAD < 4 * CT) ring[(i + LEAD) % R] = cols(i + LEAD);
+      if (i & 1) dk[t] = mma16(ring[i % R], df[t / CT], dk[t]);
+      else dv[t] = mma16(ring[i % R], pf, dv[t]);
       PIN();
     }
+  };
+  int before = 0, now = 0;
+  if (n > 0) fetch(0, 0);
+  for (int it = 0; it < n; ++it) {
+    tile_barrier<0>();
+    const int next = now + STAGE == NS * STAGE ? 0 : now + STAGE;
+    if (it + 1 < n) fetch(it + 1, next);
+    if (late && it > 0) products(before);
+    scores(now);
+    if (!late) products(now);
+    before = now;
+    now = next;
   }
+  if (late && n > 0) products(before);
   // a masked key's lane has computed with zeros for its operands and another row's statistics: it gives zeros
   const float sum = wave_sum(ok ? (float)dlam : 0.f);
   if (lane == 0) a.dlam_part[((int64_t)h * a.B + b) * (blocks * NW) + block * NW + wid] = sum;
@@ -391,7 +410,7 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   const f32x4 none = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < 2 * CT; ++t) {
-    store4(dkr + t * 16, ok ? dk[t] * a.scale : none);
+    store4(dkr + t * 16, ok ? dk[t] * (t < CT ? a.scale : -lam * a.scale) : none);
     store4(dvr + t * 16, ok ? dv[t] : none);
   }
 }
