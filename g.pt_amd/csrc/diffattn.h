@@ -116,6 +116,19 @@ __device__ __forceinline__ void operand_from(Operand& o, const f32x16& x) {   //
   }
 }
 
+// bf16: what the rounding of operand_from left of x, as a second operand (together 16 bits of mantissa)
+__device__ __forceinline__ void operand_rest(Operand& rest, const f32x16& x, const Operand& o) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const u32x4 w = __builtin_bit_cast(u32x4, o.p[s]);
+    u32x4 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = pack_bf16x2(x[8 * s + 2 * j] - __uint_as_float(w[j] << 16), x[8 * s + 2 * j + 1] - __uint_as_float(w[j] & 0xffff0000u));
+    rest.p[s] = __builtin_bit_cast(bf16x8, v);
+  }
+}
+
 // 4 consecutive values to memory
 __device__ __forceinline__ void store4(bf16_t* p, const f32x4& v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
@@ -150,9 +163,9 @@ __device__ __forceinline__ void dma_tile(const T* src, int64_t ld, int valid, ch
       off = (uint32_t)row * row_bytes + (uint32_t)((pos ^ L::f(row)) << 4);
     }
     const uint32_t more = EVEN ? (uint32_t)(c0 / NT * STEP) * row_bytes : 0u;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                      __builtin_amdgcn_readfirstlane((int)(lds + c0 * 16))),
-                 "v"(off), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane((int)more))
+                 "v"(off + more), "s"(rsrc)
                  : "memory");
   }
 }
@@ -193,9 +206,10 @@ struct ColBase {
 };
 
 // acc[column of the tile][lane's column of X] += sum over rows [row0, row0 + 32) of tile[row][..] X[row][..] for the 32 columns that
-// start at chunk C (a multiple of 4 chunks in bf16, 8 in fp32)
-template <typename T, int HD>
-__device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBase<T, HD>& cb, int row0, int C, const Operand& x, f32x16 acc) {
+// start at chunk C (a multiple of 4 chunks in bf16, 8 in fp32); rest: X's second operand, if any
+template <typename T, int HD, typename... Rest>
+__device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBase<T, HD>& cb, int row0, int C, const Operand& x, f32x16 acc,
+                                                  const Rest&... rest) {
   using L = Tile<T, HD>;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -203,7 +217,9 @@ __device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBas
       const char* p = tile + (row0 + 16 * s) * L::PITCH;
       const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + L::add(cb.lo, C)));
       const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(p + L::add(cb.hi, C)));
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), x.p[s], acc, 0, 0, 0);
+      const bf16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, x.p[s], acc, 0, 0, 0);
+      ((acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, rest.p[s], acc, 0, 0, 0)), ...);
     }
   } else {
 #pragma unroll

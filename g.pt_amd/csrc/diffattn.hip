@@ -6,21 +6,32 @@
 // so that a lane holds one query's scores (reductions over keys stay in its registers but for one exchange) and the exponentiated
 // accumulator of S^T is the operand of the second product as it stands.
 // A wave takes 32 queries and ONE map: its accumulator is 32 x 2 hd (128 registers at hd 128) where both maps' would leave one wave
-// per SIMD; the two waves of a query group join their halves through LDS at the end.  K | V tiles of 64 keys (fp32: 32) come by
+// per SIMD; the two waves of a query group join their halves through LDS at the end.  K | V tiles of 64 or 32 keys come by
 // LDS-DMA, double-buffered, one barrier per tile, and serve all waves of the workgroup.
+// P enters the second product in the operands' type.  In bf16 that rounding adds as much noise as the output's own (out is off by
+// 2.5e-3 rms at 4096 keys, 1.7e-3 if only the output is rounded; the maps' difference cancels values, not their noise).  A second
+// operand with what the first rounding left takes it away: free where memory is the bound, so done there (one query group, <= 32
+// tokens); 4096 x 4096, hd 128, 32 (sample, head) would go from 441 to 616 us for it, 515 ragged, hd 64, from 60 to 77.
 // The accumulator is rescaled only when a row's maximum has grown by more than a factor of 2^8 over the reference its sums are held
-// against: P stays below 2^8, exact in every format here.
+// against: P stays below 2^8.
 #include "diffattn.h"
 
 namespace diffattn {
 namespace {
 
-constexpr float SLACK = 8.f;   // log2 of the growth that is let pass
+constexpr float SLACK = 8.f;     // log2 of the growth that is let pass
+constexpr int MAX_SPLITS = 512;
+
+// Keys per tile.  With one query group (Tq <= 32) the kernel streams K and V: tiles of 32 keys leave a CU room for two workgroups, one
+// loading while the other computes.  1 query x 16384 keys, hd 128, 32 (sample, head): 100.7 us (5.3 TB/s), tiles of 64 keys 124.3.
+template <typename T, int NW>
+constexpr int KEYS = sizeof(T) == 2 && NW > 1 ? 64 : 32;
 
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   using L = Tile<T, HD>;
-  constexpr int NT = NW * 128, KT = sizeof(T) == 2 ? 64 : 32, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
+  constexpr int NT = NW * 128, KT = KEYS<T, NW>, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
+  constexpr bool WHOLE = sizeof(T) == 2 && NW == 1;                       // P in two bf16 operands
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [2][K | V]
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), m = wid & 1, grp = wid >> 1;
@@ -82,14 +93,14 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
     mx = col_max(mx);
     if (__any((mx - top) * a.c2 > SLACK)) {
-      const float now = fmaxf(top, mx), alpha = exp2_fast((top - now) * a.c2);
+      const float now = fmaxf(top, mx), alpha = now == -INFINITY ? 1.f : exp2_fast((top - now) * a.c2);
       top = now;
       sum *= alpha;
 #pragma unroll
       for (int t = 0; t < CT; ++t) o[t] *= alpha;
     }
-    const float ref = top * a.c2;
-    Operand p[NU];
+    const float ref = top == -INFINITY ? 0.f : top * a.c2;                   // nothing but -inf so far: exp2(-inf) = 0
+    Operand p[NU], low[WHOLE ? NU : 1];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
@@ -98,11 +109,15 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
         sum += s[u][e];
       }
       operand_from<T>(p[u], s[u]);
+      if constexpr (WHOLE) operand_rest(low[u], s[u], p[u]);
     }
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int u = 0; u < NU; ++u) o[t] = columns_product<T, HD>(tv, cb, u * 32, t * (32 * L::ES / 16), p[u], o[t]);
+      for (int u = 0; u < NU; ++u) {
+        if constexpr (WHOLE) o[t] = columns_product<T, HD>(tv, cb, u * 32, t * (32 * L::ES / 16), p[u], o[t], low[u]);
+        else o[t] = columns_product<T, HD>(tv, cb, u * 32, t * (32 * L::ES / 16), p[u], o[t]);
+      }
   }
   sum = col_sum(sum);
   if (a.splits > 1) {
@@ -151,9 +166,9 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   }
 }
 
-// joins the splits of one (sample, head, query): one wave; lane owns 4 columns of 4 hd
+// joins few splits: one wave per (sample, head, query); lane owns 4 columns of 2 hd
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void combine_kernel(Args a) {
+__global__ __launch_bounds__(256) void join_few_kernel(Args a) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (int64_t)a.B * a.H * a.Tq;
   if (row >= rows) return;
   const int lane = threadIdx.x & 63;
@@ -192,16 +207,78 @@ __global__ __launch_bounds__(256) void combine_kernel(Args a) {
   }
 }
 
-// query groups of 32 per workgroup: four share a K | V tile where that still leaves every CU a workgroup
-int groups_for(int64_t pairs, int Tq) { return Tq <= 32 ? 1 : pairs * ((Tq + 127) / 128) >= 256 || Tq > 2048 ? 4 : Tq <= 64 ? 2 : 2; }
+// joins many splits: one workgroup per (sample, head, query); each thread owns 4 columns of one map, the splits dealt out to the
+// thread groups and their shares added in group order through LDS
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void join_many_kernel(Args a) {
+  constexpr int W = 4 * HD + 4, COLS = HD, GROUPS = 256 / COLS;                // COLS threads: 4 columns each of both maps' 2 hd
+  __shared__ float weight[MAX_SPLITS][2];                                      // of a split's sums in the whole
+  __shared__ float total[2][2];                                                // top, sum of each map
+  __shared__ f32x4 share[256];
+  const int64_t row = blockIdx.x, rows = (int64_t)a.B * a.H * a.Tq;
+  const float* p = a.part + row * W;
+  const int64_t step = rows * W;
+  const int tid = threadIdx.x;
+  if (tid < 128) {                                                             // wave m: map m
+    const int lane = tid & 63, m = tid >> 6;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = lane; s < a.splits; s += 64) {
+      const float t = p[s * step + 4 * HD + 2 * m], v = p[s * step + 4 * HD + 2 * m + 1];
+      if (v == 0.f) continue;                                                  // a split without a valid key
+      const float mx = fmaxf(top, t);
+      sum = sum * exp2_fast((top - mx) * a.c2) + v * exp2_fast((t - mx) * a.c2);
+      top = mx;
+    }
+    const float all = wave_max(top);
+    sum = wave_sum(sum == 0.f ? 0.f : sum * exp2_fast((top - all) * a.c2));
+    for (int s = lane; s < a.splits; s += 64) {
+      const float v = p[s * step + 4 * HD + 2 * m + 1];
+      weight[s][m] = v == 0.f ? 0.f : exp2_fast((p[s * step + 4 * HD + 2 * m] - all) * a.c2) / sum;
+    }
+    if (lane == 0) {
+      total[m][0] = all;
+      total[m][1] = sum;
+    }
+  }
+  __syncthreads();
+  const int c = tid % COLS, grp = tid / COLS, m = c / (HD / 2);
+  if (grp < GROUPS) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = grp; s < a.splits; s += GROUPS) {
+      const float w = weight[s][m];
+      if (w != 0.f) acc += *reinterpret_cast<const f32x4*>(p + s * step + c * 4) * w;   // (a weight of 0: sums that hold nothing, or nothing left of them)
+    }
+    share[tid] = acc;
+  }
+  __syncthreads();
+  const int qi = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
+  if (tid < HD / 2) {
+    f32x4 first = share[tid], second = share[tid + HD / 2];
+#pragma unroll
+    for (int q = 1; q < GROUPS; ++q) {
+      first += share[q * COLS + tid];
+      second += share[q * COLS + tid + HD / 2];
+    }
+    store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD + tid * 4, first - second * a.lam[h]);
+    if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD + tid * 4, second);
+  }
+  if (a.lse && tid < 2) {
+    const float s = total[tid][1];
+    a.lse[(((int64_t)tid * a.B + b) * a.H + h) * a.Tq + qi] = s == 0.f ? INFINITY : total[tid][0] * a.c2 + __builtin_amdgcn_logf(s);
+  }
+}
 
-// spans of keys per (sample, head, query block): as many as give 256 CUs a workgroup each, none shorter than 256 keys
+// query groups of 32 per workgroup: four share a K | V tile where that still leaves every CU a workgroup
+int groups_for(int64_t pairs, int Tq) { return Tq <= 32 ? 1 : pairs * ((Tq + 127) / 128) >= 256 ? 4 : 2; }
+
+// spans of keys per (sample, head, query block): as many as give 256 CUs a workgroup each (two of the small ones), none shorter than
+// 256 keys
 int splits_for(int B, int Tq, int Tk, int H) {
   const int64_t pairs = (int64_t)B * H;
   const int nw = groups_for(pairs, Tq);
   const int64_t wgs = pairs * ((Tq + 32 * nw - 1) / (32 * nw));
   if (wgs >= 192) return 1;
-  const int64_t want = 256 / wgs, most = (Tk + 255) / 256;
+  const int64_t want = (nw == 1 ? MAX_SPLITS : 256) / wgs, most = (Tk + 255) / 256;
   return (int)(want < most ? want : most);
 }
 
@@ -212,7 +289,7 @@ int launch_nw(const Args& a, hipStream_t s) {
   if (int st = grant_lds(fwd_kernel<T, HD, NW>, once, who)) return st;
   const int64_t grid = (int64_t)a.B * a.H * a.splits * ((a.Tq + 32 * NW - 1) / (32 * NW));
   GPT_REQUIRE(grid * NW * 128 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
-  constexpr int LDS = 4 * (sizeof(T) == 2 ? 64 : 32) * Tile<T, HD>::PITCH;
+  constexpr int LDS = 4 * KEYS<T, NW> * Tile<T, HD>::PITCH;
   static_assert(NW * 2 * HD / 32 * 4 * 64 * 16 <= LDS, "the hand-over of the second map's halves has to fit the tiles' LDS");
   hipLaunchKernelGGL((fwd_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 128), LDS, s, a);
   return gpt_launch_status(who);
@@ -224,7 +301,12 @@ int launch(const Args& a, hipStream_t s) {
   if (int st = nw == 4 ? launch_nw<T, HD, 4>(a, s) : nw == 2 ? launch_nw<T, HD, 2>(a, s) : launch_nw<T, HD, 1>(a, s)) return st;
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.B * a.H * a.Tq;
-    hipLaunchKernelGGL((combine_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    // few splits come with many rows, where a wave each is enough: 2 splits x 4112 rows (hd 96, fp32) 7.0 us, a workgroup each 11.2;
+    // 64 splits x 32 rows (hd 128) go through a wave one after another, 12.6 us, a workgroup 4.9
+    if (a.splits < 8)
+      hipLaunchKernelGGL((join_few_kernel<T, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((join_many_kernel<T, HD>), dim3((unsigned)rows), dim3(256), 0, s, a);
     return gpt_launch_status("gpt_diff_attention");
   }
   return 0;

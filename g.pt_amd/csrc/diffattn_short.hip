@@ -1,9 +1,10 @@
 // Differential attention over Tq, Tk <= 32 tokens (the denoiser's own sequences: 18 and 26), forward and backward: one wave per
 // (sample, head), everything between loads and stores in registers and the wave's own LDS.
 //
-// The operands arrive by LDS-DMA (buffer loads: rows behind the sample's end lie outside the buffer's range and arrive as zeros),
-// once each, in rows of 2 hd elements; 16-byte chunk c of row r is stored at chunk c ^ f(r), with f such that 16 rows read at one
-// chunk hit 16 different 16-byte bank groups and the 4 rows of a transposing read 4 different 64-byte ones.
+// Each operand is read once.  What is used by rows only (the forward's K, the backward's V) goes straight to registers, the others to
+// LDS by DMA (buffer loads: rows behind the sample's end lie outside the buffer's range and arrive as zeros), in rows of 2 hd
+// elements; the outputs leave through the tiles of operands that are done with.  16-byte chunk c of row r is stored at chunk
+// c ^ f(r), with f such that the lanes that LDS serves together hit different banks, by rows as well as in transposing reads.
 // 32 x 32 tiles: S_i^T = K_i Q_i^T and dP^T = V dO^T with keys on the accumulator's rows and queries on its lanes: softmax and
 // D_i = sum P_i dP are sums over a lane's registers and one exchange, in fp32 throughout.  The backward takes both transposed uses
 // (dQ contracts over keys, dK and dV over queries) from one evaluation: dS_i^T is dQ's operand as it stands in the registers; dS_i
@@ -45,9 +46,9 @@ __device__ __forceinline__ f32x16 rows_product(const char* ta, bool ina, const c
 }
 
 // acc^T[column 32 t + i of the tile][lane's column of X] = sum over the tile's rows (n valid) of tile[row][..] X[row][..].  ORDER of the
-// rows in the operand: 0 = an accumulator's (operand_from), 1 = ascending (bf16: 16 s + 8 hh + j; fp32: 2 e + hh)
-template <typename T, int HD, int ORDER>
-__device__ __forceinline__ f32x16 columns_product(const char* tile, int n, int t, const Operand& x, int lane, const char* zero) {
+// rows in the operand: 0 = an accumulator's (operand_from), 1 = ascending (bf16: 16 s + 8 hh + j; fp32: 2 e + hh).  rest: X's second operand, if any
+template <typename T, int HD, int ORDER, typename... Rest>
+__device__ __forceinline__ f32x16 columns_product(const char* tile, int n, int t, const Operand& x, int lane, const char* zero, const Rest&... rest) {
   using L = Tile<T, HD>;
   f32x16 acc = zero16();
   if constexpr (sizeof(T) == 2) {
@@ -58,7 +59,9 @@ __device__ __forceinline__ f32x16 columns_product(const char* tile, int n, int t
       const int r0 = 16 * s + (ORDER ? 8 : 4) * hh + tq, r1 = r0 + (ORDER ? 4 : 8);
       const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(r0 < n ? tile + L::at(r0, chunk) + in : zero));
       const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(r1 < n ? tile + L::at(r1, chunk) + in : zero));
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), x.p[s], acc, 0, 0, 0);
+      const bf16x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, x.p[s], acc, 0, 0, 0);
+      ((acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, rest.p[s], acc, 0, 0, 0)), ...);
     }
   } else {
     const int r = lane & 31, hh = lane >> 5, col = t * 32 + r;
@@ -155,14 +158,17 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 3 : 1) void short_fwd_kernel(A
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m) softmax32(s[m], len, hh, a.c2);
-  Operand p;
+  Operand p, rest;
 #pragma unroll
   for (int e = 0; e < 16; ++e) s[0][e] -= lam * s[1][e];
-  operand_from<T>(p, s[0]);                                 // bf16: the difference of the maps is rounded, once
+  operand_from<T>(p, s[0]);                                 // the difference of the maps; bf16: in two operands, 16 bits
+  if constexpr (sizeof(T) == 2) operand_rest(rest, s[0], p);
   lds_done();                                               // Q has been read: its tile takes the output
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const f32x16 o = columns_product<T, HD, 0>(tv, a.Tk, t, p, lane, zero);
+    f32x16 o;
+    if constexpr (sizeof(T) == 2) o = columns_product<T, HD, 0>(tv, a.Tk, t, p, lane, zero, rest);
+    else o = columns_product<T, HD, 0>(tv, a.Tk, t, p, lane, zero);
     if (qok) stage<T, HD>(tq, r, hh, t, o, 1.f);
   }
   lds_done();

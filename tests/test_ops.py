@@ -511,6 +511,21 @@ def test_diff_attention_garbage_behind_the_lengths(T, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", [BF, F32])
+@pytest.mark.parametrize("Tq,Tk,gone", [(20, 26, 9), (40, 200, 130), (1, 700, 300), (5, 9000, 8200)])
+def test_diff_attention_scores_of_minus_infinity(Tq, Tk, gone, t):
+    """Keys whose scores are -inf weigh nothing, also where they fill the first tiles or a whole span of the keys."""
+    _, q, k, v, lam, _, _ = attention_case(2, Tq, Tk, 2, 64, t, None, False)
+    q, k = q.view(2, Tq, 4, 64), k.view(2, Tk, 4, 64)
+    q[..., 7], k[:, :gone, :, 7] = 1.0, -math.inf
+    q, k = q.view(2, Tq, -1), k.view(2, Tk, -1)
+    want, tol = attention_reference(q, k[:, gone:], v[:, gone:], lam, 2, None, 64 ** -0.5, None, 0.0 if t == F32 else HALF[t])
+    got = ops.diff_attention(q, k, v, lam, 2)
+    extra = (gone + 4) * U * want["out"].abs()           # the longer sums' adds of zeros round nothing, but their count is counted
+    within(got, want["out"], tol["out"] + extra + HALF[t] * (want["out"].abs() + tol["out"]))
+
+
+@gpu
 @pytest.mark.parametrize("T", [20, 90])
 def test_diff_attention_nan_stays_in_its_sample(T):
     _, q, k, v, lam, n, g = attention_case(3, T, T, 2, 64, BF, None, False)
