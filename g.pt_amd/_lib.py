@@ -67,6 +67,10 @@ class Dropout(C.Structure):
     _fields_ = [("p", f64), ("seed", u64), ("offset", u64), ("offset_dev", vp)]
 
 
+class DenoiserDropout(C.Structure):
+    _fields_ = [("embd", f64), ("attn", f64), ("resid", f64), ("seed", u64), ("offset", u64), ("offset_dev", vp)]
+
+
 class AddRmsNorm(C.Structure):
     _fields_ = [(n, i32) for n in ("h_dtype", "x_dtype", "y_dtype")] + \
                [("h", vp), ("ldh", i64), ("resid", vp), ("ldr", i64), ("x_out", vp), ("ldx", i64), ("weight", vp), ("y", vp), ("ldy", i64),
@@ -136,6 +140,12 @@ _PROTOS = {
     "gpt_denoiser_backward": ([C.POINTER(Model), C.POINTER(Workspace), C.POINTER(Backward), vp, vp, vp, i32, vp], i32),
     "gpt_denoiser_backward_stages": ([C.POINTER(Model), C.POINTER(Workspace), C.POINTER(Backward), vp, vp, vp, i32, i32, i32,
                                       vp], i32),
+    "gpt_denoiser_forward_dropout": ([C.POINTER(Model), C.POINTER(Workspace), C.POINTER(DenoiserDropout), vp, vp, vp, vp, i32, vp, vp,
+                                      i32, vp], i32),
+    "gpt_denoiser_backward_stages_dropout": ([C.POINTER(Model), C.POINTER(Workspace), C.POINTER(Backward), C.POINTER(DenoiserDropout),
+                                              vp, vp, vp, i32, i32, i32, vp], i32),
+    "gpt_attention_dropout": ([i32, vp, vp, i32, i32, i32, i32, i32, C.POINTER(Dropout), vp], i32),
+    "gpt_attention_dropout_bwd": ([i32, vp, vp, vp, i32, i32, i32, i32, C.POINTER(Dropout), vp], i32),
     "gpt_ddim_reverse_step": ([vp, vp, vp, vp, vp, i32, i32, i32, f32, f32, vp, vp, i32, i32, vp], i32),
     "gpt_prior_bpd": ([vp, f32, f32, vp, i32, i32, vp], i32),
     "gpt_pair_gather": ([vp, i64, i64, vp, vp, vp, C.c_float, vp, vp, i32, i32, vp], i32),

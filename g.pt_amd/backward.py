@@ -198,15 +198,17 @@ def _descriptor(eng, buf, scratch, overwrite=False, defer=1, sumsq=None):
 
 
 def forward_keep(model, x, t, lt, lp, x_prev):
-    """Training forward: keeps per-layer activations and LayerNorm statistics in the engine's workspace."""
+    """Training forward: keeps per-layer activations and LayerNorm statistics in the engine's workspace, and in eng.drop what the
+    backward needs to draw this forward's dropout masks again (None: no dropout)."""
     eng = model.engine(x.device)
     _ensure_training_state(eng)
     B = x.shape[0]
     ws = eng.workspace(B, keep_activations=True)
     eng.keep_gen += 1
+    eng.drop = model.draw_dropout()
     out = torch.empty_like(x)
-    L.check(L.lib().gpt_denoiser_forward(C.byref(eng.cmodel), C.byref(ws), L.ptr(x), L.ptr(t), L.ptr(lt), L.ptr(lp),
-                                         int(lt.dtype == torch.float64), L.ptr(x_prev), L.ptr(out), B, L.stream()),
+    L.check(L.lib().gpt_denoiser_forward_dropout(C.byref(eng.cmodel), C.byref(ws), eng.drop, L.ptr(x), L.ptr(t), L.ptr(lt), L.ptr(lp),
+                                                 int(lt.dtype == torch.float64), L.ptr(x_prev), L.ptr(out), B, L.stream()),
             "gpt_denoiser_forward")
     return eng, ws, out
 
@@ -230,8 +232,8 @@ def backward_into(eng, ws, x, x_prev, d_out, buf, schedule=None, overwrite=False
     done = 0
     for stage_end, callback in list(schedule or []) + [(n_stages, None)]:
         if stage_end > done:
-            L.check(L.lib().gpt_denoiser_backward_stages(C.byref(eng.cmodel), C.byref(ws), C.byref(bw), L.ptr(x), L.ptr(x_prev),
-                                                         L.ptr(d_out), B, done, stage_end, L.stream()),
+            L.check(L.lib().gpt_denoiser_backward_stages_dropout(C.byref(eng.cmodel), C.byref(ws), C.byref(bw), eng.drop, L.ptr(x),
+                                                                 L.ptr(x_prev), L.ptr(d_out), B, done, stage_end, L.stream()),
                     "gpt_denoiser_backward_stages")
             done = stage_end
         if callback is not None:
@@ -265,7 +267,7 @@ class _PendingBackward:
         # before this backward overwrites them (or re-allocates them for a larger batch).  The generation counter turns that
         # into an error instead of silently wrong gradients; the buffers stay referenced here so that a re-allocation cannot
         # free memory this backward's descriptor still points at.
-        self.keep_gen, self.bufs = eng.keep_gen, eng.buffers(keep_activations=True)
+        self.keep_gen, self.bufs, self.drop = eng.keep_gen, eng.buffers(keep_activations=True), eng.drop
         self.versions = tuple(p._version for p in model.parameters())
         self.buf = self.bw = self.keep = self.d_out = None
         self.done = 0
@@ -284,9 +286,9 @@ class _PendingBackward:
 
     def run_stage(self, stage):
         assert stage == self.done, "backward stages run in order"
-        L.check(L.lib().gpt_denoiser_backward_stages(C.byref(self.eng.cmodel), C.byref(self.ws), C.byref(self.bw), L.ptr(self.x),
-                                                     L.ptr(self.x_prev), L.ptr(self.d_out), self.x.shape[0], stage, stage + 1,
-                                                     L.stream()), "gpt_denoiser_backward_stages")
+        L.check(L.lib().gpt_denoiser_backward_stages_dropout(C.byref(self.eng.cmodel), C.byref(self.ws), C.byref(self.bw), self.drop,
+                                                             L.ptr(self.x), L.ptr(self.x_prev), L.ptr(self.d_out), self.x.shape[0],
+                                                             stage, stage + 1, L.stream()), "gpt_denoiser_backward_stages")
         self.done = stage + 1
 
 

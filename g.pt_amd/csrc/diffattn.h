@@ -60,7 +60,8 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 //   a transposing read serves 32 lanes: 4 rows x 64 bytes, or 8 rows x 32 (neighbouring quads in different halves).
 template <typename T, int HD>
 struct Tile {
-  static constexpr int ES = sizeof(T), PITCH = 2 * HD * ES, CPR = PITCH / 16, CM = CPR / 2;   // bytes per row, chunks per row and per map
+  static constexpr int ES = sizeof(T), COLS = 2 * HD, PITCH = COLS * ES, CPR = PITCH / 16, CM = CPR / 2;   // bytes per row, chunks per row and per map
+  static constexpr int REAL = CPR;
   static constexpr int MASK = PITCH % 256 == 0 ? 15 : 7;
   __device__ static __forceinline__ int f(int r) {
     const int b0 = (r >> 2) & 1, b1 = (r >> 3) & 1, pair = ((b0 ^ b1) << 1) | b1;   // quads of rows 0, 1, 2, 3 -> 0, 2, 3, 1

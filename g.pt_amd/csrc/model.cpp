@@ -54,11 +54,26 @@ static bool prune_last_train(const gpt_model_t* m, int B) {
   return on && m->dtype == GPT_BF16 && m->n_layer > 0 && To < T && m->d % 256 == 0;
 }
 
-static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, const float* x, const int64_t* t,
+// Dropout of a training step (gpt_denoiser_dropout_t): the masks' sites, 0 = embeddings, then three per Block
+enum { SITE_ATTN = 1, SITE_PROJ = 2, SITE_MLP = 3 };
+static gpt_dropout_t drop_site(const gpt_denoiser_dropout_t* d, double p, int site) {
+  return gpt_dropout_t{p, d->seed, d->offset + (uint64_t)site, d->offset_dev};
+}
+static int check_drop(const gpt_denoiser_dropout_t** d, const char* who) {
+  if (!*d) return 0;
+  for (double p : {(*d)->embd, (*d)->attn, (*d)->resid}) GPT_REQUIRE(p >= 0.0 && p <= 1.0, "%s: dropout probability %g not in [0, 1]", who, p);
+  GPT_REQUIRE((uintptr_t)(*d)->offset_dev % 8 == 0, "%s: misaligned device counter", who);
+  if ((*d)->embd == 0.0 && (*d)->attn == 0.0 && (*d)->resid == 0.0) *d = nullptr;
+  return 0;
+}
+
+static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_denoiser_dropout_t* drop, const float* x, const int64_t* t,
                             const void* loss_target, const void* loss_prev, int loss_is_f64, const float* x_prev, float* out,
                             int B, int enc_cached, void* stream) {
   CHECK(validate(m, ws, B, "gpt_denoiser_forward"));
   GPT_REQUIRE(x && t && loss_target && loss_prev && x_prev && out, "gpt_denoiser_forward: null operand");
+  CHECK(check_drop(&drop, "gpt_denoiser_forward"));
+  const bool embd_drop = drop && drop->embd > 0.0, attn_drop = drop && drop->attn > 0.0, resid_drop = drop && drop->resid > 0.0;
   const int d = m->d, T = m->T, M = B * T, L = m->n_layer, dt = m->dtype;
   const size_t es = esize(dt);
   const int W = 2 * m->nfreq + 1;
@@ -99,16 +114,20 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
     const char* e = getenv("GPT_PRUNE_LAST");   // 0: all rows through the last Block (cross-check, A/B)
     return !e || atoi(e) != 0;
   }();
-  const bool prune = prune_on && !keep && L > 0 && m->n_out_tok < T && (size_t)(T - m->n_out_tok) * 4 * es >= (size_t)m->n_out_tok * 4;
+  const bool prune = prune_on && !keep && !drop && L > 0 && m->n_out_tok < T && (size_t)(T - m->n_out_tok) * 4 * es >= (size_t)m->n_out_tok * 4;
 
   // ln_in + position embedding (transformer.py:226, 308-309), then the first Block's ln1: one launch in the inference forward
   // (no statistics kept), two otherwise
   static const bool ln_pair = [] { const char* e = getenv("GPT_LN_FUSE0"); return !e || atoi(e) != 0; }();   // 0: two launches (A/B)
-  if (ln_pair && !keep && L > 0 && gpt_layernorm_pair_has(d)) {
+  if (ln_pair && !keep && !embd_drop && L > 0 && gpt_layernorm_pair_has(d)) {
     CHECK(gpt_layernorm_pair(ws->enc, m->ln_in_w, m->ln_in_b, m->pos_emb, T, xbuf(0), m->layers[0].ln1_w, m->layers[0].ln1_b,
                              lay(ws->h1, 0, d), dt, M, d, 1e-5f, stream));
   } else {
     CHECK(gpt_layernorm(ws->enc, m->ln_in_w, m->ln_in_b, m->pos_emb, T, xbuf(0), GPT_F32, stat(0, 0), stat(0, 1), M, d, 1e-5f, stream));
+    if (embd_drop) {
+      const gpt_dropout_t site = drop_site(drop, drop->embd, 0);
+      CHECK(gpt_dropout_add(GPT_F32, xbuf(0), d, GPT_F32, nullptr, 0, xbuf(0), d, M, d, &site, stream));
+    }
     // Every residual Linear is launched together with the LayerNorm that reads its result (gpt_gemm_resadd_layernorm: one
     // fused pass at small batches, the two kernels otherwise): proj + ln2, mlp.2 + the next block's ln1 (ln_f after the last).
     CHECK(gpt_layernorm(xbuf(0), m->layers[0].ln1_w, m->layers[0].ln1_b, nullptr, 0, lay(ws->h1, 0, d), dt, stat(1, 0), stat(1, 1), M, d,
@@ -127,16 +146,31 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
     CHECK(wait_ready(ly.ready, stream));
     CHECK(gpt_gemm_nt(dt, h1, d, ly.wqkv, d, ly.bqkv, qkv, 3 * d, nullptr, 0, M, 3 * d, d, GPT_EPI_STORE, stream));
     const bool last = l + 1 == L;
+    auto attention = [&](int t_out) -> int {
+      if (!attn_drop) return gpt_attention_rows(dt, qkv, att, B, T, t_out, m->n_head, d / m->n_head, stream);
+      const gpt_dropout_t site = drop_site(drop, drop->attn, 3 * l + SITE_ATTN);
+      return gpt_attention_dropout(dt, qkv, att, B, T, t_out, m->n_head, d / m->n_head, &site, stream);
+    };
+    // xo = xr + dropout(A . W^T + b), then the LayerNorm that reads xo.  With dropout three launches: the Linear's fp32 output waits
+    // in a buffer that is free by then (kept activations: xout, whose turn comes last; else the attention's inputs)
+    auto residual = [&](int which, const void* A, int K, const void* W, const float* bias, const float* xr, float* xo, const float* nw,
+                        const float* nb, void* nh, float* mean, float* rstd, int rows) -> int {
+      if (!resid_drop)
+        return gpt_gemm_resadd_layernorm(dt, A, K, W, K, bias, xr, d, xo, d, nw, nb, nh, mean, rstd, rows, d, K, 1e-5f, stream);
+      const gpt_dropout_t site = drop_site(drop, drop->resid, 3 * l + which);
+      float* f = keep ? xout : reinterpret_cast<float*>(ws->qkv);
+      CHECK(gpt_gemm_nt(dt, A, K, W, K, bias, f, d, nullptr, 0, rows, d, K, GPT_EPI_STORE_F32, stream));
+      CHECK(gpt_dropout_add(GPT_F32, f, d, GPT_F32, xr, d, xo, d, rows, d, &site, stream));
+      return gpt_layernorm(xo, nw, nb, nullptr, 0, nh, dt, mean, rstd, rows, d, 1e-5f, stream);
+    };
     if (last && keep && prune_last_train(m, B)) {
       const int To = m->n_out_tok, Mc = B * To;
       void* pre = lay(ws->pre, l, 4 * (size_t)d);
-      CHECK(gpt_attention_rows(dt, qkv, att, B, T, To, m->n_head, d / m->n_head, stream));
+      CHECK(attention(To));
       CHECK(gpt_gather_token_rows(xin, xmid, B, T, To, d, stream));                 // compact residual rows: [B * To, d]
-      CHECK(gpt_gemm_resadd_layernorm(dt, att, d, ly.wproj, d, ly.bproj, xmid, d, xmid, d, ly.ln2_w, ly.ln2_b, h2, stat(2 + 2 * l, 0),
-                                      stat(2 + 2 * l, 1), Mc, d, d, 1e-5f, stream));
+      CHECK(residual(SITE_PROJ, att, d, ly.wproj, ly.bproj, xmid, xmid, ly.ln2_w, ly.ln2_b, h2, stat(2 + 2 * l, 0), stat(2 + 2 * l, 1), Mc));
       CHECK(gpt_gemm_nt(dt, h2, d, ly.w1, d, ly.b1, act, 4 * d, pre, 4 * d, Mc, 4 * d, d, GPT_EPI_GELU_AUX, stream));
-      CHECK(gpt_gemm_resadd_layernorm(dt, act, 4 * d, ly.w2, 4 * d, ly.b2, xmid, d, xout, d, m->ln_f_w, m->ln_f_b, ws->hf, stat(2 * L + 1, 0),
-                                      stat(2 * L + 1, 1), Mc, d, 4 * d, 1e-5f, stream));
+      CHECK(residual(SITE_MLP, act, 4 * d, ly.w2, ly.b2, xmid, xout, m->ln_f_w, m->ln_f_b, ws->hf, stat(2 * L + 1, 0), stat(2 * L + 1, 1), Mc));
       CHECK(wait_ready(m->dec_ready, stream));
       return gpt_decode_tokens(dt, To, ws->hf, To, m->dec_w, m->dec_n, m->dec_off, x_prev, out, B, d, m->D, stream);
     }
@@ -158,9 +192,8 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
       CHECK(wait_ready(m->dec_ready, stream));
       return gpt_decode_tokens(dt, To, ws->hf, To, m->dec_w, m->dec_n, m->dec_off, x_prev, out, B, d, m->D, stream);
     }
-    CHECK(gpt_attention(dt, qkv, att, B, T, m->n_head, d / m->n_head, stream));
-    CHECK(gpt_gemm_resadd_layernorm(dt, att, d, ly.wproj, d, ly.bproj, xin, d, xmid, d, ly.ln2_w, ly.ln2_b, h2, stat(2 + 2 * l, 0),
-                                    stat(2 + 2 * l, 1), M, d, d, 1e-5f, stream));
+    CHECK(attention(T));
+    CHECK(residual(SITE_PROJ, att, d, ly.wproj, ly.bproj, xin, xmid, ly.ln2_w, ly.ln2_b, h2, stat(2 + 2 * l, 0), stat(2 + 2 * l, 1), M));
     if (keep) {
       void* pre = lay(ws->pre, l, 4 * (size_t)d);
       CHECK(gpt_gemm_nt(dt, h2, d, ly.w1, d, ly.b1, act, 4 * d, pre, 4 * d, M, 4 * d, d, GPT_EPI_GELU_AUX, stream));
@@ -171,8 +204,7 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
     const float* nb = last ? m->ln_f_b : m->layers[l + 1].ln1_b;
     void* nh = last ? ws->hf : lay(ws->h1, l + 1, d);
     const int ns = last ? 2 * L + 1 : 1 + 2 * (l + 1);
-    CHECK(gpt_gemm_resadd_layernorm(dt, act, 4 * d, ly.w2, 4 * d, ly.b2, xmid, d, xout, d, nw, nb, nh, stat(ns, 0), stat(ns, 1), M, d,
-                                    4 * d, 1e-5f, stream));
+    CHECK(residual(SITE_MLP, act, 4 * d, ly.w2, ly.b2, xmid, xout, nw, nb, nh, stat(ns, 0), stat(ns, 1), M));
   }
   CHECK(wait_ready(m->dec_ready, stream));
   CHECK(gpt_decode_tokens(dt, m->n_out_tok, ws->hf, T, m->dec_w, m->dec_n, m->dec_off, x_prev, out, B, d, m->D, stream));
@@ -182,7 +214,13 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
 extern "C" int gpt_denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, const float* x, const int64_t* t,
                                     const void* loss_target, const void* loss_prev, int loss_is_f64,
                                     const float* x_prev, float* out, int B, void* stream) {
-  return denoiser_forward(m, ws, x, t, loss_target, loss_prev, loss_is_f64, x_prev, out, B, 0, stream);
+  return denoiser_forward(m, ws, nullptr, x, t, loss_target, loss_prev, loss_is_f64, x_prev, out, B, 0, stream);
+}
+
+extern "C" int gpt_denoiser_forward_dropout(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_denoiser_dropout_t* drop, const float* x,
+                                            const int64_t* t, const void* loss_target, const void* loss_prev, int loss_is_f64,
+                                            const float* x_prev, float* out, int B, void* stream) {
+  return denoiser_forward(m, ws, drop, x, t, loss_target, loss_prev, loss_is_f64, x_prev, out, B, 0, stream);
 }
 
 // ddim: 0 = ancestral DDPM step (gpt_posterior_step), 1 = DDIM step with `eta` (gpt_ddim_step, needs alphas_cumprod)
@@ -210,7 +248,7 @@ static int sample_loop(const char* who, int ddim, float eta, const float* alphas
     // (the fused posterior kernel of step i + 1 has written this step's model timesteps already)
     if (!fused_post || i == first_step) CHECK(gpt_fill_i64(t_model, B, host_timestep_map[i], stream));
     // x_prev and the losses are the loop's constants: their tokens are encoded in the first step only
-    CHECK(denoiser_forward(m, ws, x, t_model, loss_target, loss_prev, loss_is_f64, x_prev, model_out, B, i != first_step, stream));
+    CHECK(denoiser_forward(m, ws, nullptr, x, t_model, loss_target, loss_prev, loss_is_f64, x_prev, model_out, B, i != first_step, stream));
     if (fused_post) {
       // DDPM with in-kernel noise: Philox + posterior update in one kernel, the timestep as a scalar
       CHECK(gpt_posterior_step_philox(model_out, x, i, coef, predict_xstart, use_clamp, lo, hi, seed, (uint64_t)i, x, B, m->D,
@@ -263,11 +301,19 @@ extern "C" int gpt_denoiser_backward(const gpt_model_t* m, const gpt_workspace_t
 extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_backward_t* bw,
                                             const float* x, const float* x_prev, const float* d_out, int B, int stage_begin,
                                             int stage_end, void* stream) {
+  return gpt_denoiser_backward_stages_dropout(m, ws, bw, nullptr, x, x_prev, d_out, B, stage_begin, stage_end, stream);
+}
+
+extern "C" int gpt_denoiser_backward_stages_dropout(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_backward_t* bw,
+                                                    const gpt_denoiser_dropout_t* drop, const float* x, const float* x_prev,
+                                                    const float* d_out, int B, int stage_begin, int stage_end, void* stream) {
   CHECK(validate(m, ws, B, "gpt_denoiser_backward"));
   GPT_REQUIRE(0 <= stage_begin && stage_begin < stage_end && stage_end <= m->n_layer + 2,
               "gpt_denoiser_backward_stages: bad stage range [%d, %d) of %d", stage_begin, stage_end, m->n_layer + 2);
   GPT_REQUIRE(bw && bw->layers && x && x_prev && d_out, "gpt_denoiser_backward: null operand");
   GPT_REQUIRE(ws->layer_stride == 1, "gpt_denoiser_backward: needs the workspace of a training forward");
+  CHECK(check_drop(&drop, "gpt_denoiser_backward"));
+  const bool embd_drop = drop && drop->embd > 0.0, attn_drop = drop && drop->attn > 0.0, resid_drop = drop && drop->resid > 0.0;
   const int d = m->d, T = m->T, M = B * T, L = m->n_layer, dt = m->dtype;
   const size_t es = esize(dt);
   const size_t Mmax = (size_t)ws->B_max * T;
@@ -287,10 +333,17 @@ extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_work
     const char* e = getenv("GPT_DGELU_COLSUM");   // 0: mlp.0's bias gradient by a separate gpt_colsum launch (cross-check, A/B)
     return !e || atoi(e) != 0;
   }();
-  static const bool fuse_col = [] {
+  static const bool fuse_col_on = [] {
     const char* e = getenv("GPT_LNB_COLSUM");   // 0: bias gradients of mlp.2 / attn.proj by separate gpt_colsum launches (cross-check, A/B)
     return !e || atoi(e) != 0;
   }();
+  // With dropout behind the Linears, dY of a Linear is not the residual stream's gradient but that times the mask: `masked` forms it
+  // (in the compute type, from the fp32 gradient the LayerNorm backward left), and the bias gradients are its column sums
+  const bool fuse_col = fuse_col_on && !resid_drop;
+  auto masked = [&](int site_no, const float* g, void* gt, int rows) -> int {
+    const gpt_dropout_t site = drop_site(drop, drop->resid, site_no);
+    return gpt_dropout_add(GPT_F32, g, d, dt, nullptr, 0, gt, d, rows, d, &site, stream);
+  };
   // LayerNorm backward: per-workgroup sums into bw->ln_partials where there is room (one reduce launch at the end of this call),
   // float atomics otherwise
   LnPartCalls ln_calls;
@@ -350,8 +403,9 @@ extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_work
   // bw->g / bw->gt = gradient of the residual stream behind the last Block = dY of its mlp.2: the bias gradient g_b2 is its column sum,
   // taken by the LayerNorm backward that produces it (and so for every Block below: ln1's backward of Block l + 1 feeds Block l's mlp.2,
   // ln2's backward feeds the attention projection of its own Block)
-  CHECK(ln_bwd(bw->d_tok, GPT_F32, xbuf(2 * L), stat(2 * L + 1, 0), stat(2 * L + 1, 1), m->ln_f_w, nullptr, bw->g, bw->gt,
-               dt, bw->g_ln_f_w, bw->g_ln_f_b, fuse_col && L > 0 ? bw->layers[L - 1].g_b2 : nullptr, Mc));
+  CHECK(ln_bwd(bw->d_tok, GPT_F32, xbuf(2 * L), stat(2 * L + 1, 0), stat(2 * L + 1, 1), m->ln_f_w, nullptr, bw->g,
+               resid_drop ? nullptr : bw->gt, dt, bw->g_ln_f_w, bw->g_ln_f_b, fuse_col && L > 0 ? bw->layers[L - 1].g_b2 : nullptr, Mc));
+  if (resid_drop) CHECK(masked(3 * (L - 1) + SITE_MLP, bw->g, bw->gt, Mc));
   }
 
   // stages 1 .. L - the blocks, last to first (stage s = layer L - s)
@@ -413,8 +467,9 @@ extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_work
     CHECK(gpt_gemm_nt(dt, d_act_l, 4 * d, gl.w1_t, 4 * d, nullptr, bw->d_h, d, nullptr, 0, Ml, d, 4 * d, GPT_EPI_STORE, stream));
     // (compact rows: the residual gradient leaves this LayerNorm backward in bw->d_tok, free between stage 0 and stage L + 1, and
     // is scattered back to all rows below)
-    CHECK(ln_bwd(bw->d_h, dt, xbuf(2 * l + 1), stat(2 + 2 * l, 0), stat(2 + 2 * l, 1), ly.ln2_w, bw->g, cmp ? bw->d_tok : bw->g, gt2, dt,
-                 gl.g_ln2_w, gl.g_ln2_b, fuse_col ? gl.g_bproj : nullptr, Ml));
+    CHECK(ln_bwd(bw->d_h, dt, xbuf(2 * l + 1), stat(2 + 2 * l, 0), stat(2 + 2 * l, 1), ly.ln2_w, bw->g, cmp ? bw->d_tok : bw->g,
+                 resid_drop ? nullptr : gt2, dt, gl.g_ln2_w, gl.g_ln2_b, fuse_col ? gl.g_bproj : nullptr, Ml));
+    if (resid_drop) CHECK(masked(3 * l + SITE_PROJ, cmp ? bw->d_tok : bw->g, gt2, Ml));
     // attention output projection
     if (!fuse_col) CHECK(gpt_colsum(dt, gt2, d, gl.g_bproj, Ml, d, stream));
     if (!grouped) CHECK(wgrad(gt2, d, att, d, gl.g_wproj));
@@ -427,7 +482,12 @@ extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_work
       CHECK(gpt_scatter_token_rows(bw->d_tok, bw->g, B, T, To, d, 4, stream));
       d_att = bw->tB;
     }
-    CHECK(gpt_attention_bwd(dt, qkv, d_att, d_qkv_l, B, T, m->n_head, d / m->n_head, stream));
+    if (attn_drop) {
+      const gpt_dropout_t site = drop_site(drop, drop->attn, 3 * l + SITE_ATTN);
+      CHECK(gpt_attention_dropout_bwd(dt, qkv, d_att, d_qkv_l, B, T, m->n_head, d / m->n_head, &site, stream));
+    } else {
+      CHECK(gpt_attention_bwd(dt, qkv, d_att, d_qkv_l, B, T, m->n_head, d / m->n_head, stream));
+    }
     // query | key | value
     CHECK(gpt_colsum(dt, d_qkv_l, 3 * d, gl.g_bqkv, M, 3 * d, stream));
     if (grouped) {
@@ -447,12 +507,17 @@ extern "C" int gpt_denoiser_backward_stages(const gpt_model_t* m, const gpt_work
       CHECK(wgrad(d_qkv_l, 3 * d, h1, d, gl.g_wqkv));
     }
     CHECK(gpt_gemm_nt(dt, d_qkv_l, 3 * d, gl.wqkv_t, 3 * d, nullptr, bw->d_h, d, nullptr, 0, M, d, 3 * d, GPT_EPI_STORE, stream));
-    CHECK(ln_bwd(bw->d_h, dt, xbuf(2 * l), stat(1 + 2 * l, 0), stat(1 + 2 * l, 1), ly.ln1_w, bw->g, bw->g, gt_next, dt,
-                 gl.g_ln1_w, gl.g_ln1_b, fuse_col && l > 0 ? bw->layers[l - 1].g_b2 : nullptr, M));
+    CHECK(ln_bwd(bw->d_h, dt, xbuf(2 * l), stat(1 + 2 * l, 0), stat(1 + 2 * l, 1), ly.ln1_w, bw->g, bw->g,
+                 resid_drop ? nullptr : gt_next, dt, gl.g_ln1_w, gl.g_ln1_b, fuse_col && l > 0 ? bw->layers[l - 1].g_b2 : nullptr, M));
+    if (resid_drop && l > 0) CHECK(masked(3 * (l - 1) + SITE_MLP, bw->g, gt_next, M));
   }
   CHECK(flush());                                        // what this call collected (gradients are complete when it returns)
   if (stage_end < L + 2) return gpt_ln_partials_reduce(ln_calls, d, stream);
   // stage L + 1 - position embedding: sum over the batch of the gradient of x0 = ln_in(enc) + pos_emb
+  if (embd_drop) {
+    const gpt_dropout_t site = drop_site(drop, drop->embd, 0);
+    CHECK(gpt_dropout_add(GPT_F32, bw->g, d, GPT_F32, nullptr, 0, bw->g, d, M, d, &site, stream));
+  }
   CHECK(gpt_colsum(GPT_F32, bw->g, (int64_t)T * d, bw->g_pos_emb, B, T * d, stream));
   CHECK(ln_bwd(bw->g, GPT_F32, ws->enc, stat(0, 0), stat(0, 1), m->ln_in_w, nullptr, bw->d_tok, nullptr, GPT_F32,
                bw->g_ln_in_w, bw->g_ln_in_b, nullptr, M));

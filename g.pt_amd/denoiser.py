@@ -13,6 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
+from . import dp
 
 
 # ------------------------------------------------------------------------------------------ token plan
@@ -132,6 +133,7 @@ class GPT(nn.Module):
             nn.Sequential(nn.Linear(n_embd, n, bias=False)) for n in self.output_splits)
         self.num_output_heads = len(self.output_splits)
         self.n_embd, self.n_head, self.n_layer = n_embd, n_head, n_layer
+        self.embd_pdrop, self.attn_pdrop, self.resid_pdrop = embd_pdrop, attn_pdrop, resid_pdrop
         self.dropout_p = max(attn_pdrop, resid_pdrop, embd_pdrop)
         self.apply(self._init_weights)
 
@@ -521,11 +523,18 @@ class Gpt(nn.Module):
             lt, lp = lt.double(), lp.double()
         return x, t, lt, lp, x_prev
 
+    def draw_dropout(self):
+        """The dropout masks of one forward in training mode (transformer.py:27-28, 66, 219): probabilities, and a seed drawn from
+        torch's CPU generator, so torch.manual_seed makes runs repeatable; every rank takes offsets of its own.  None without dropout."""
+        dec = self.decoder
+        if not self.training or dec.dropout_p <= 0:
+            return None
+        seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
+        return L.DenoiserDropout(dec.embd_pdrop, dec.attn_pdrop, dec.resid_pdrop, seed, dp.get_rank() * (3 * dec.n_layer + 1), None)
+
     def forward(self, x, t, loss_target, loss_prev=None, x_prev=None):
         """(N, D) denoised parameters; same contract as transformer.py:440-464."""
         needs_grad = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
-        if self.training and self.decoder.dropout_p > 0:
-            raise NotImplementedError("dropout > 0 is not implemented on the HIP path (every shipped config uses 0)")
         x, t, lt, lp, x_prev = self._prepare(x, t, loss_target, loss_prev, x_prev)
         if x.shape[0] == 0:                       # an empty batch: the reference returns an empty (0, D) tensor; no launch
             return torch.empty_like(x)
@@ -536,7 +545,8 @@ class Gpt(nn.Module):
         B = x.shape[0]
         ws = eng.workspace(B)
         out = torch.empty_like(x)
-        L.check(L.lib().gpt_denoiser_forward(C.byref(eng.cmodel), C.byref(ws), L.ptr(x), L.ptr(t), L.ptr(lt), L.ptr(lp),
-                                             int(lt.dtype == torch.float64), L.ptr(x_prev), L.ptr(out), B, L.stream()),
+        L.check(L.lib().gpt_denoiser_forward_dropout(C.byref(eng.cmodel), C.byref(ws), self.draw_dropout(), L.ptr(x), L.ptr(t), L.ptr(lt),
+                                                     L.ptr(lp), int(lt.dtype == torch.float64), L.ptr(x_prev), L.ptr(out), B,
+                                                     L.stream()),
                 "gpt_denoiser_forward")
         return out

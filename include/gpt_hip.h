@@ -624,6 +624,31 @@ typedef struct {
 int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes);
 int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_diff_attention_bwd_t* g, void* stream);
 
+/* ---- dropout in the denoiser's training step ------------------------------------------------------------------------------------
+ * gpt_attention_rows with dropout on the softmax probabilities (Gpt/models/transformer.py:45-46), and its backward (dqkv is stored):
+ * element (((sample * n_head + head) * T + query) * 32 + key) of the mask.  T <= 32, hd 32, 64, 96 or 128. */
+int gpt_attention_dropout(int dtype, const void* qkv, void* y, int B, int T, int t_out, int n_head, int hd, const gpt_dropout_t* drop,
+                          void* stream);
+int gpt_attention_dropout_bwd(int dtype, const void* qkv, const void* dy, void* dqkv, int B, int T, int n_head, int hd,
+                              const gpt_dropout_t* drop, void* stream);
+
+/* The probabilities of transformer.py:27-28, 66, 219 (embd: position-embedded tokens; attn: attention probabilities; resid: the
+ * outputs of both residual branches of a Block).  The masks of a step take the offsets offset .. offset + 3 n_layer: site 0 = embd,
+ * 1 + 3 l, 2 + 3 l, 3 + 3 l = Block l's attention, projection and MLP; forward and backward of a step are given the same struct.
+ * (Where the last Block works on the decoded tokens' rows alone, its two residual masks are those of the compact rows.) */
+typedef struct {
+  double embd, attn, resid;
+  uint64_t seed, offset;
+  const uint64_t* offset_dev;            /* device counter added to offset, or NULL (see gpt_dropout_t) */
+} gpt_denoiser_dropout_t;
+/* gpt_denoiser_forward / gpt_denoiser_backward_stages of a model in training mode; drop NULL or all zeros: exactly those. */
+int gpt_denoiser_forward_dropout(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_denoiser_dropout_t* drop, const float* x,
+                                 const int64_t* t, const void* loss_target, const void* loss_prev, int loss_is_f64,
+                                 const float* x_prev, float* out, int B, void* stream);
+int gpt_denoiser_backward_stages_dropout(const gpt_model_t* m, const gpt_workspace_t* ws, const gpt_backward_t* bw,
+                                         const gpt_denoiser_dropout_t* drop, const float* x, const float* x_prev, const float* d_out,
+                                         int B, int stage_begin, int stage_end, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
