@@ -243,12 +243,13 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// workgroup -> (pair, block of the pair): all blocks of a (sample, head) on one XCD, whose L2 then holds the rows they share
+// workgroup -> (pair, block of the pair).  All blocks of a (sample, head) on one XCD (workgroups go round them), whose L2 then holds the
+// rows they share, and the pairs dealt out in turn: samples of different lengths spread over the XCDs.  The last pairs % 8 are not.
 __device__ __forceinline__ void xcd_block(int id, int n, int per_pair, int* pair, int* block) {
-  const int q8 = n >> 3, r8 = n & 7, x = id & 7;
-  const int idx = (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + (id >> 3);
-  *pair = idx / per_pair;
-  *block = idx - *pair * per_pair;
+  const int whole = n / per_pair / 8 * 8 * per_pair, j = id < whole ? id >> 3 : id;
+  const int p = j / per_pair;
+  *pair = id < whole ? p * 8 + (id & 7) : p;
+  *block = j - p * per_pair;
 }
 
 // max / sum over the two lanes that hold one column of a 32 x 32 accumulator

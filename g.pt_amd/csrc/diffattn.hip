@@ -70,6 +70,7 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   for (int it = 0; it < n; ++it) {
     tile_barrier<0>();                                                     // tile `it` is here, the other buffer has been read
     if (it + 1 < n) fetch(it + 1);
+    if (block * 32 * NW + grp * 32 >= a.Tq) continue;                       // a wave without a query only loads
     const char *tk = smem + (it & 1) * 2 * TILE, *tv = tk + TILE;
     f32x16 s[NU];
 #pragma unroll

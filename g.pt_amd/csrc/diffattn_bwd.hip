@@ -434,6 +434,10 @@ int64_t key_tiles(int Tk) { return ((int64_t)Tk + 127) / 128 * 8; }
 // four, which may have 512 registers each (eight would spill)
 template <typename T, int HD>
 constexpr int MANY = sizeof(T) == 4 && HD >= 96 ? 4 : 8;
+// dK / dV in bf16 at hd 64: 170 registers, so three waves per SIMD in workgroups of four, two in workgroups of eight (4 x 4096 tokens,
+// 8 heads: 787 and 835 us; 16 samples of up to 515: 58 and 65.  At hd 32, 4 x 4096: 490 and 459; hd 128, T = 4096: 1034 and 636)
+template <typename T, int HD>
+constexpr int MANY_KEYS = sizeof(T) == 2 && HD == 64 ? 4 : MANY<T, HD>;
 bool many_waves(int64_t pairs, int T) { return T > 32 && pairs * ((T + 127) / 128) >= 192; }
 
 template <typename T, int HD, int NW>
@@ -465,9 +469,9 @@ int launch(const Args& a, f32x4* stats, float* dlam, hipStream_t s) {
   GPT_REQUIRE(nd < (1ll << 24), "%s: too many rows (%lld)", who, (long long)rows);
   hipLaunchKernelGGL((stats_kernel<T, HD>), dim3((unsigned)nd), dim3(256), 0, s, a, stats);
   if (int st = gpt_launch_status(who)) return st;
-  constexpr int M = MANY<T, HD>;
-  const int nk = many_waves(pairs, a.Tk) ? M : 2;
-  if (int st = nk == M ? launch_dkv<T, HD, M>(a, s) : launch_dkv<T, HD, 2>(a, s)) return st;
+  constexpr int M = MANY<T, HD>, MK = MANY_KEYS<T, HD>;
+  const int nk = many_waves(pairs, a.Tk) ? MK : 2;
+  if (int st = nk == MK ? launch_dkv<T, HD, MK>(a, s) : launch_dkv<T, HD, 2>(a, s)) return st;
   if (int st = many_waves(pairs, a.Tq) ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, 2>(a, s)) return st;
   const int64_t tiles = ((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk;
   hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, (int64_t)a.B * tiles, dlam);
