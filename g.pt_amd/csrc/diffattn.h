@@ -24,7 +24,10 @@ struct Args {
   void *dq, *dk, *dv;
   int64_t lddq, bsdq, lddk, bsdk, lddv, bsdv;
   const f32x4* stats;         // [B][H][Tq]: lse_1, lse_2, D_1, D_2
-  float* dlam_part;           // [H][B * key tiles]
+  float* dlam_part;           // [H][B * splits * key tiles]
+  // split sweeps: spans of q_tiles / k_tiles tiles of 32, sums of a span [span][B * H][Tq or Tk][2 hd]
+  int q_splits, q_tiles, k_splits, k_tiles;
+  float *dq_part, *dk_part, *dv_part;
 };
 
 // Tq, Tk <= 32 (diffattn_short.hip); the backward needs dlam_part [H][B], no lse, out, out2 or delta

@@ -273,13 +273,13 @@ __global__ __launch_bounds__(256) void join_many_kernel(Args a) {
 int groups_for(int64_t pairs, int Tq) { return Tq <= 32 ? 1 : pairs * ((Tq + 127) / 128) >= 256 ? 4 : 2; }
 
 // spans of keys per (sample, head, query block): as many as give 256 CUs a workgroup each (two of the small ones), none shorter than
-// 256 keys
-int splits_for(int B, int Tq, int Tk, int H) {
+// 256 keys (fp32, where a key costs eight times as much: 128)
+int splits_for(int dtype, int B, int Tq, int Tk, int H) {
   const int64_t pairs = (int64_t)B * H;
   const int nw = groups_for(pairs, Tq);
   const int64_t wgs = pairs * ((Tq + 32 * nw - 1) / (32 * nw));
   if (wgs >= 192) return 1;
-  const int64_t want = (nw == 1 ? MAX_SPLITS : 256) / wgs, most = (Tk + 255) / 256;
+  const int64_t want = (nw == 1 ? MAX_SPLITS : 256) / wgs, least = dtype == GPT_BF16 ? 256 : 128, most = (Tk + least - 1) / least;
   return (int)(want < most ? want : most);
 }
 
@@ -352,16 +352,16 @@ int make_args(const gpt_diff_attention_t* p, const char* who, Args* a) {
 
 using namespace diffattn;
 
-static int64_t fwd_workspace(int B, int Tq, int Tk, int n_head, int hd) {
+static int64_t fwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd) {
   if (Tq <= SHORT && Tk <= SHORT) return 0;
-  const int n = splits_for(B, Tq, Tk, n_head);
+  const int n = splits_for(dtype, B, Tq, Tk, n_head);
   return n > 1 ? (int64_t)n * B * n_head * Tq * (4 * hd + 4) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int gpt_diff_attention_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes) {
   GPT_REQUIRE(host_bytes && (dtype == GPT_F32 || dtype == GPT_BF16) && B > 0 && Tq > 0 && Tk > 0 && n_head > 0 && hd > 0,
               "gpt_diff_attention_workspace: bad arguments");
-  *host_bytes = fwd_workspace(B, Tq, Tk, n_head, hd);
+  *host_bytes = fwd_workspace(dtype, B, Tq, Tk, n_head, hd);
   return 0;
 }
 
@@ -370,10 +370,10 @@ extern "C" int gpt_diff_attention(const gpt_diff_attention_t* p, void* stream) {
   Args a;
   if (int st = make_args(p, who, &a)) return st;
   if (p->Tq <= SHORT && p->Tk <= SHORT) return short_attention(a, p->dtype, p->hd, false, (hipStream_t)stream);
-  const int64_t need = fwd_workspace(p->B, p->Tq, p->Tk, p->n_head, p->hd);
+  const int64_t need = fwd_workspace(p->dtype, p->B, p->Tq, p->Tk, p->n_head, p->hd);
   if (need > 0) {
     GPT_REQUIRE(p->ws && (uintptr_t)p->ws % 16 == 0 && p->ws_bytes >= need, "%s: needs %lld bytes of scratch", who, (long long)need);
-    const int n = splits_for(p->B, p->Tq, p->Tk, p->n_head);
+    const int n = splits_for(p->dtype, p->B, p->Tq, p->Tk, p->n_head);
     a.part = (float*)p->ws;
     a.splits = n;
     a.split_keys = ((p->Tk + n - 1) / n + 63) / 64 * 64;

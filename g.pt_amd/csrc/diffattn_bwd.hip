@@ -183,7 +183,9 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (a.Tq + 16 * NW - 1) / (16 * NW);
   int pair, block;
-  xcd_block(blockIdx.x, gridDim.x, blocks, &pair, &block);
+  xcd_block(blockIdx.x, gridDim.x, blocks * a.k_splits, &pair, &block);
+  const int split = block / blocks;
+  block -= split * blocks;
   const int b = pair / a.H, h = pair - b * a.H, len = valid_keys(a, b);
   const T* kb = (const T*)a.k + (int64_t)b * a.bsk + h * 2 * HD;
   const T* vb = (const T*)a.v + (int64_t)b * a.bsv + h * 2 * HD;
@@ -205,9 +207,10 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 #pragma unroll
   for (int t = 0; t < 2 * CT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int rb = row16_base<T, HD>(lane), cb = col16_base<T, HD>(lane);
-  const int n = (len + 31) / 32;
+  const int first = split * a.k_tiles, n = min((len + 31) / 32 - first, a.k_tiles);   // tiles of this span
   auto fetch = [&](int it, int at) {
     char* dst = smem + at;
+    it += first;
     dma_tile<T, HD, 32, NT>(kb + (int64_t)it * 32 * a.ldk, a.ldk, len - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(vb + (int64_t)it * 32 * a.ldv, a.ldv, len - it * 32, dst + TILE, tid, wid);
   };
@@ -245,6 +248,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[m][u][r] = exp2_fast(s[m][u][r] * a.c2 - st[m]) * (dp[u][r] - st[2 + m]);
+    it += first;
     if (it * 32 + 32 > len) {
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -284,9 +288,12 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
   }
   if (late && n > 0) products(before);
   if (!qok) return;
-  T* dq = (T*)a.dq + (int64_t)b * a.bsdq + (int64_t)qi * a.lddq + h * 2 * HD + 4 * g;
+  auto store = [&](auto* dq) {
 #pragma unroll
-  for (int t = 0; t < 2 * CT; ++t) store4(dq + t * 16, acc[t] * (t < CT ? a.scale : -lam * a.scale));   // -lam of dS_2: here, once
+    for (int t = 0; t < 2 * CT; ++t) store4(dq + t * 16, acc[t] * (t < CT ? a.scale : -lam * a.scale));   // -lam of dS_2: here, once
+  };
+  if (a.k_splits > 1) store(a.dq_part + (((int64_t)split * a.B * a.H + pair) * a.Tq + qi) * (2 * HD) + 4 * g);
+  else store((T*)a.dq + (int64_t)b * a.bsdq + (int64_t)qi * a.lddq + h * 2 * HD + 4 * g);
 }
 
 // dK, dV and the tile's share of sum P_2 dP: NW waves of 16 keys; Q | dO | statistics tiles of 32 queries.  S_i = Q_i K_i^T and
@@ -300,7 +307,9 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (a.Tk + 16 * NW - 1) / (16 * NW);
   int pair, block;
-  xcd_block(blockIdx.x, gridDim.x, blocks, &pair, &block);
+  xcd_block(blockIdx.x, gridDim.x, blocks * a.q_splits, &pair, &block);
+  const int split = block / blocks;
+  block -= split * blocks;
   const int b = pair / a.H, h = pair - b * a.H, len = valid_keys(a, b);
   const T* qb = (const T*)a.q + (int64_t)b * a.bsq + h * 2 * HD;
   const T* gb = (const T*)a.dout + (int64_t)b * a.bsdo + h * 2 * HD;
@@ -323,9 +332,11 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   for (int t = 0; t < 2 * CT; ++t) dk[t] = dv[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   double dlam = 0.0;
   const int rb = row16_base<T, HD>(lane), cb = col16_base<T, HD>(lane);
-  const int n = block * NW * 16 < len ? (a.Tq + 31) / 32 : 0;               // a block without a valid key: zeros
+  const int first = split * a.q_tiles;
+  const int n = block * NW * 16 < len ? min((a.Tq + 31) / 32 - first, a.q_tiles) : 0;   // a block without a valid key: zeros
   auto fetch = [&](int it, int at) {
     char* dst = smem + at;
+    it += first;
     dma_tile<T, HD, 32, NT>(qb + (int64_t)it * 32 * a.ldq, a.ldq, a.Tq - it * 32, dst, tid, wid);
     dma_tile<T, HD, 32, NT>(gb + (int64_t)it * 32 * a.lddo, a.lddo, a.Tq - it * 32, dst + TILE, tid, wid);
     if (wid == 0) dma_bytes(sb + it * 32, (a.Tq - it * 32) * 16, dst + 2 * TILE, lane);
@@ -403,16 +414,46 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   if (late && n > 0) products(before);
   // a masked key's lane has computed with zeros for its operands and another row's statistics: it gives zeros
   const float sum = wave_sum(ok ? (float)dlam : 0.f);
-  if (lane == 0) a.dlam_part[((int64_t)h * a.B + b) * (blocks * NW) + block * NW + wid] = sum;
+  if (lane == 0) a.dlam_part[(((int64_t)h * a.B + b) * a.q_splits + split) * (blocks * NW) + block * NW + wid] = sum;
   if (key >= a.Tk) return;
-  T* dkr = (T*)a.dk + (int64_t)b * a.bsdk + (int64_t)key * a.lddk + h * 2 * HD + 4 * g;
-  T* dvr = (T*)a.dv + (int64_t)b * a.bsdv + (int64_t)key * a.lddv + h * 2 * HD + 4 * g;
-  const f32x4 none = {0.f, 0.f, 0.f, 0.f};
+  auto store = [&](auto* dkr, auto* dvr) {
+    const f32x4 none = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int t = 0; t < 2 * CT; ++t) {
-    store4(dkr + t * 16, ok ? dk[t] * (t < CT ? a.scale : -lam * a.scale) : none);
-    store4(dvr + t * 16, ok ? dv[t] : none);
+    for (int t = 0; t < 2 * CT; ++t) {
+      store4(dkr + t * 16, ok ? dk[t] * (t < CT ? a.scale : -lam * a.scale) : none);
+      store4(dvr + t * 16, ok ? dv[t] : none);
+    }
+  };
+  if (a.q_splits > 1) {
+    const int64_t at = (((int64_t)split * a.B * a.H + pair) * a.Tk + key) * (2 * HD) + 4 * g;
+    store(a.dk_part + at, a.dv_part + at);
+  } else {
+    store((T*)a.dk + (int64_t)b * a.bsdk + (int64_t)key * a.lddk + h * 2 * HD + 4 * g,
+          (T*)a.dv + (int64_t)b * a.bsdv + (int64_t)key * a.lddv + h * 2 * HD + 4 * g);
   }
+}
+
+// the spans' sums of dQ (where the keys were split) and of dK, dV (where the queries were), added in the spans' order: a thread owns 4
+// columns of a row
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  constexpr int W = 2 * HD, PER = W / 4;
+  const int64_t pairs = (int64_t)a.B * a.H, nq = a.k_splits > 1 ? pairs * a.Tq : 0, nk = a.q_splits > 1 ? pairs * a.Tk : 0;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int64_t row = i / PER;
+  const int c = (int)(i - row * PER) * 4;
+  if (row >= nq + 2 * nk) return;
+  const bool is_q = row < nq, is_k = !is_q && row < nq + nk;
+  row -= is_q ? 0 : is_k ? nq : nq + nk;
+  const int n = is_q ? a.Tq : a.Tk, splits = is_q ? a.k_splits : a.q_splits;
+  const float* p = (is_q ? a.dq_part : is_k ? a.dk_part : a.dv_part) + row * W + c;
+  const int64_t step = (is_q ? nq : nk) * W;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+  for (int s = 1; s < splits; ++s) sum += *reinterpret_cast<const f32x4*>(p + s * step);
+  const int64_t pair = row / n, t = row - pair * n;
+  const int64_t b = pair / a.H, h = pair - b * a.H;
+  T* out = (T*)(is_q ? a.dq : is_k ? a.dk : a.dv) + b * (is_q ? a.bsdq : is_k ? a.bsdk : a.bsdv) + t * (is_q ? a.lddq : is_k ? a.lddk : a.lddv);
+  store4(out + h * W + c, sum);
 }
 
 // dlam[h] = -(sum of the head's partial sums): one workgroup per head, each thread every 256th in index order, then a fixed tree
@@ -427,24 +468,57 @@ __global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ par
   if (threadIdx.x == 0) dlam[blockIdx.x] = -((red[0] + red[1]) + (red[2] + red[3]));
 }
 
-// partial sums of dlam per (head, sample): one per 16 keys of the workgroups' blocks
-int64_t key_tiles(int Tk) { return ((int64_t)Tk + 127) / 128 * 8; }
-
-// waves of 16 rows per workgroup: eight share the tiles where that still gives every CU a workgroup, else two.  fp32 from hd 96 on:
-// four, which may have 512 registers each (eight would spill)
+// waves of 16 rows per workgroup: eight share the tiles where that still gives every CU a workgroup; fp32 from hd 96 on: four, which may
+// have 512 registers each (eight would spill)
 template <typename T, int HD>
 constexpr int MANY = sizeof(T) == 4 && HD >= 96 ? 4 : 8;
 // dK / dV in bf16 at hd 64: 170 registers, so three waves per SIMD in workgroups of four, two in workgroups of eight (4 x 4096 tokens,
 // 8 heads: 787 and 835 us; 16 samples of up to 515: 58 and 65.  At hd 32, 4 x 4096: 490 and 459; hd 128, T = 4096: 1034 and 636)
 template <typename T, int HD>
 constexpr int MANY_KEYS = sizeof(T) == 2 && HD == 64 ? 4 : MANY<T, HD>;
+// ... else four, one per SIMD: two workgroups of two waves share SIMDs while others idle (32 (sample, head) x 512 tokens, hd 128: dK / dV
+// and dQ 47 and 42 us in bf16, 43 and 31 by fours; in fp32 180 and 226, 168 and 126)
+constexpr int FEW = 4;
 bool many_waves(int64_t pairs, int T) { return T > 32 && pairs * ((T + 127) / 128) >= 192; }
+
+// How a call is cut.  Workgroups of four waves that do not fill the CUs have their sweep split into spans, up to one workgroup per CU
+// (two where registers and LDS leave room: hd <= 64), whose sums are joined by a launch of their own (6 to 10 us): worth it from 5
+// tiles of 32 rows per span in bf16 and, the matrix rate being an eighth there, from 2 in fp32.  dK / dV and dQ, unsplit and split:
+// 16 (sample, head) x 257 tokens, hd 96, fp32: 67 and 52 us, 32 and 24; 2 x 2048, hd 128, bf16: 130 and 106, 42 and 32.
+struct Plan {
+  bool many_q, many_k;
+  int q_splits = 1, q_tiles, k_splits = 1, k_tiles;
+  int64_t stats, dlam, dq, dkv;                                            // bytes of the workspace's parts (dkv: each of the two)
+  int64_t bytes() const { return stats + dlam + dq + 2 * dkv; }
+};
+int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
+void spans(int64_t wgs, int64_t fill, int tiles, int least, int* splits, int* per) {
+  const int64_t want = fill / wgs, most = tiles / least, n = want < most ? want : most;
+  *per = n > 1 ? (int)((tiles + n - 1) / n) : tiles;
+  *splits = (tiles + *per - 1) / *per;
+}
+Plan plan_for(int dtype, int B, int Tq, int Tk, int H, int hd) {
+  Plan p;
+  const int64_t pairs = (int64_t)B * H;
+  const int qt = (Tq + 31) / 32, kt = (Tk + 31) / 32, least = dtype == GPT_BF16 ? 5 : 2, fill = hd <= 64 ? 512 : 256;
+  p.many_q = many_waves(pairs, Tq);
+  p.many_k = many_waves(pairs, Tk);
+  p.q_tiles = qt;
+  p.k_tiles = kt;
+  if (!p.many_k) spans(pairs * ((kt + 1) / 2), fill, qt, least, &p.q_splits, &p.q_tiles);
+  if (!p.many_q) spans(pairs * ((qt + 1) / 2), fill, kt, least, &p.k_splits, &p.k_tiles);
+  p.stats = 16 * pairs * Tq;
+  p.dlam = round16(pairs * p.q_splits * (((int64_t)Tk + 127) / 128 * 8) * 4);   // one per 16 keys of the workgroups' blocks
+  p.dq = p.k_splits > 1 ? pairs * p.k_splits * Tq * 2 * hd * 4 : 0;
+  p.dkv = p.q_splits > 1 ? pairs * p.q_splits * Tk * 2 * hd * 4 : 0;
+  return p;
+}
 
 template <typename T, int HD, int NW>
 int launch_dq(const Args& a, hipStream_t s) {
   const char* who = "gpt_diff_attention_bwd";
   static GptPerDevice once;
-  const int64_t grid = ((int64_t)a.Tq + 16 * NW - 1) / (16 * NW) * a.H * a.B;
+  const int64_t grid = ((int64_t)a.Tq + 16 * NW - 1) / (16 * NW) * a.k_splits * a.H * a.B;
   GPT_REQUIRE(grid * NW * 64 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
   if (int st = grant_lds(dq_kernel<T, HD, NW>, once, who)) return st;
   hipLaunchKernelGGL((dq_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 64), (STAGES<T, NW> * 64 * Tile<T, HD>::PITCH), s, a);
@@ -455,7 +529,7 @@ template <typename T, int HD, int NW>
 int launch_dkv(const Args& a, hipStream_t s) {
   const char* who = "gpt_diff_attention_bwd";
   static GptPerDevice once;
-  const int64_t grid = ((int64_t)a.Tk + 16 * NW - 1) / (16 * NW) * a.H * a.B;
+  const int64_t grid = ((int64_t)a.Tk + 16 * NW - 1) / (16 * NW) * a.q_splits * a.H * a.B;
   GPT_REQUIRE(grid * NW * 64 < (1ll << 32) && grid < (1ll << 31), "%s: too many workgroups (%lld)", who, (long long)grid);
   if (int st = grant_lds(dkv_kernel<T, HD, NW>, once, who)) return st;
   hipLaunchKernelGGL((dkv_kernel<T, HD, NW>), dim3((unsigned)grid), dim3(NW * 64), (STAGES<T, NW> * (64 * Tile<T, HD>::PITCH + 512)), s, a);
@@ -463,37 +537,40 @@ int launch_dkv(const Args& a, hipStream_t s) {
 }
 
 template <typename T, int HD>
-int launch(const Args& a, f32x4* stats, float* dlam, hipStream_t s) {
+int launch(const Args& a, const Plan& plan, f32x4* stats, float* dlam, hipStream_t s) {
   const char* who = "gpt_diff_attention_bwd";
-  const int64_t rows = (int64_t)a.B * a.Tq * a.H, nd = (rows + 15) / 16, pairs = (int64_t)a.B * a.H;
+  const int64_t pairs = (int64_t)a.B * a.H, rows = pairs * a.Tq, nd = (rows + 15) / 16;
   GPT_REQUIRE(nd < (1ll << 24), "%s: too many rows (%lld)", who, (long long)rows);
   hipLaunchKernelGGL((stats_kernel<T, HD>), dim3((unsigned)nd), dim3(256), 0, s, a, stats);
   if (int st = gpt_launch_status(who)) return st;
   constexpr int M = MANY<T, HD>, MK = MANY_KEYS<T, HD>;
-  const int nk = many_waves(pairs, a.Tk) ? MK : 2;
-  if (int st = nk == MK ? launch_dkv<T, HD, MK>(a, s) : launch_dkv<T, HD, 2>(a, s)) return st;
-  if (int st = many_waves(pairs, a.Tq) ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, 2>(a, s)) return st;
-  const int64_t tiles = ((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk;
-  hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, (int64_t)a.B * tiles, dlam);
+  if (int st = plan.many_k ? launch_dkv<T, HD, MK>(a, s) : launch_dkv<T, HD, FEW>(a, s)) return st;
+  if (int st = plan.many_q ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, FEW>(a, s)) return st;
+  const int64_t joined = ((a.k_splits > 1 ? rows : 0) + (a.q_splits > 1 ? 2 * pairs * a.Tk : 0)) * (HD / 2);
+  if (joined > 0) {
+    hipLaunchKernelGGL((join_kernel<T, HD>), dim3((unsigned)((joined + 255) / 256)), dim3(256), 0, s, a);
+    if (int st = gpt_launch_status(who)) return st;
+  }
+  const int nk = plan.many_k ? MK : FEW;
+  const int64_t parts = (int64_t)a.B * a.q_splits * (((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk);
+  hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, parts, dlam);
   return gpt_launch_status(who);
 }
-
-int64_t round16(int64_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace
 }  // namespace diffattn
 
 using namespace diffattn;
 
-static int64_t bwd_workspace(int B, int Tq, int Tk, int n_head) {
+static int64_t bwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd) {
   if (Tq <= SHORT && Tk <= SHORT) return round16((int64_t)n_head * B * 4);
-  return (int64_t)16 * B * n_head * Tq + round16((int64_t)n_head * B * key_tiles(Tk) * 4);
+  return plan_for(dtype, B, Tq, Tk, n_head, hd).bytes();
 }
 
 extern "C" int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes) {
   GPT_REQUIRE(host_bytes && (dtype == GPT_F32 || dtype == GPT_BF16) && B > 0 && Tq > 0 && Tk > 0 && n_head > 0 && hd > 0,
               "gpt_diff_attention_bwd_workspace: bad arguments");
-  *host_bytes = bwd_workspace(B, Tq, Tk, n_head);
+  *host_bytes = bwd_workspace(dtype, B, Tq, Tk, n_head, hd);
   return 0;
 }
 
@@ -512,7 +589,7 @@ extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_d
   GPT_REQUIRE(rows_ok(p->dout, p->lddo, p->bsdo, f->Tq, false) && rows_ok(p->dq, p->lddq, p->bsdq, f->Tq, true) &&
                   rows_ok(p->dk, p->lddk, p->bsdk, f->Tk, true) && rows_ok(p->dv, p->lddv, p->bsdv, f->Tk, true),
               "%s: gradient rows must be 16-byte aligned, a row's width or more apart", who);
-  const int64_t need = bwd_workspace(f->B, f->Tq, f->Tk, f->n_head);
+  const int64_t need = bwd_workspace(f->dtype, f->B, f->Tq, f->Tk, f->n_head, f->hd);
   GPT_REQUIRE(p->ws && (uintptr_t)p->ws % 16 == 0 && p->ws_bytes >= need, "%s: needs %lld bytes of scratch", who, (long long)need);
   a.dout = p->dout; a.lddo = p->lddo; a.bsdo = p->bsdo;
   a.dq = p->dq; a.lddq = p->lddq; a.bsdq = p->bsdq;
@@ -525,15 +602,21 @@ extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_d
     hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, (int64_t)a.B, p->dlam);
     return gpt_launch_status(who);
   }
+  const Plan plan = plan_for(f->dtype, f->B, f->Tq, f->Tk, f->n_head, f->hd);
   f32x4* stats = (f32x4*)p->ws;
   a.stats = stats;
-  a.dlam_part = (float*)((char*)p->ws + (int64_t)16 * f->B * f->n_head * f->Tq);
+  a.dlam_part = (float*)((char*)p->ws + plan.stats);
+  a.dq_part = (float*)((char*)a.dlam_part + plan.dlam);
+  a.dk_part = (float*)((char*)a.dq_part + plan.dq);
+  a.dv_part = (float*)((char*)a.dk_part + plan.dkv);
+  a.q_splits = plan.q_splits; a.q_tiles = plan.q_tiles;
+  a.k_splits = plan.k_splits; a.k_tiles = plan.k_tiles;
 #define GO(T)                                          \
   switch (f->hd) {                                     \
-    case 32: return launch<T, 32>(a, stats, p->dlam, s);  \
-    case 64: return launch<T, 64>(a, stats, p->dlam, s);  \
-    case 96: return launch<T, 96>(a, stats, p->dlam, s);  \
-    default: return launch<T, 128>(a, stats, p->dlam, s); \
+    case 32: return launch<T, 32>(a, plan, stats, p->dlam, s);  \
+    case 64: return launch<T, 64>(a, plan, stats, p->dlam, s);  \
+    case 96: return launch<T, 96>(a, plan, stats, p->dlam, s);  \
+    default: return launch<T, 128>(a, plan, stats, p->dlam, s); \
   }
   if (f->dtype == GPT_BF16) GO(bf16_t)
   GO(float)

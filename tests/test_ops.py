@@ -526,6 +526,15 @@ def test_diff_attention_scores_of_minus_infinity(Tq, Tk, gone, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", [BF, F32])
+@pytest.mark.parametrize("Tq,Tk,hd", [(600, 600, 64), (40, 2000, 128), (2000, 40, 96), (333, 1025, 32)])
+def test_diff_attention_long_sweeps_of_few_heads(Tq, Tk, hd, t):
+    """Few (sample, head) pairs: the sweeps over keys and over queries are cut into spans whose sums are joined; lengths end within a
+    span, before one, at a tile's edge and at nothing."""
+    check_attention(4, Tq, Tk, 1, hd, t, lens=[Tk, 0, Tk // 2 + 1, 32])
+
+
+@gpu
 @pytest.mark.parametrize("T", [20, 90])
 def test_diff_attention_nan_stays_in_its_sample(T):
     _, q, k, v, lam, n, g = attention_case(3, T, T, 2, 64, BF, None, False)
