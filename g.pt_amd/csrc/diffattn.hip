@@ -101,17 +101,19 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
       for (int t = 0; t < CT; ++t) o[t] *= alpha;
     }
     const float ref = top == -INFINITY ? 0.f : top * a.c2;                   // nothing but -inf so far: exp2(-inf) = 0
+    float part = 0.f;                                                       // the tile's sum first: chains of 32 and of n additions, not 32 n
     Operand p[NU], low[WHOLE ? NU : 1];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[u][e] = exp2_fast(s[u][e] * a.c2 - ref);
-        sum += s[u][e];
+        part += s[u][e];
       }
       operand_from<T>(p[u], s[u]);
       if constexpr (WHOLE) operand_rest(low[u], s[u], p[u]);
     }
+    sum += part;
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll

@@ -35,6 +35,16 @@ __device__ __forceinline__ void frag_zero(Frag<float>& f) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) f.v[j] = 0.f;
 }
+__device__ __forceinline__ void frag_negate(Frag<bf16_t>& f) {
+  u32x4 w = __builtin_bit_cast(u32x4, f.v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] ^= 0x80008000u;
+  f.v = __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ void frag_negate(Frag<float>& f) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f.v[j] = -f.v[j];
+}
 // block c of 32 elements of the row at p (16-byte aligned), zeros where !ok: lane group g takes 8 consecutive ones in bf16, two
 // 16-byte chunks four apart in fp32 (as row16 reads them)
 __device__ __forceinline__ Frag<bf16_t> frag_row(const bf16_t* p, int c, int g, bool ok) {
@@ -324,8 +334,12 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     for (int c = 0; c < 2 * KC; ++c) {
       kf[c] = frag_row(kr, c, g, ok);
       vf[c] = frag_row(vr, c, g, ok);
+      if (wid & 1) frag_negate(vf[c]);
     }
   }
+  // The matrix unit's sums lean down by some 2^-32 of their terms' size: next to nothing, but dlam is what nearly cancelling terms leave
+  // (at 4 x 4096 x 4096 of them the lean is 1e-6 of it).  Every other wave takes -V and so has the lean of -dP.
+  const float sign = wid & 1 ? -1.f : 1.f;
   const float lam = a.lam[h];
   f32x4 dk[2 * CT], dv[2 * CT];
 #pragma unroll
@@ -373,10 +387,11 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       for (int r = 0; r < 4; ++r) {
         const f32x4 st = ts[16 * u + r];
         const float p0 = exp2_fast(s[0][u][r] * a.c2 - st[0]), p1 = exp2_fast(s[1][u][r] * a.c2 - st[1]);
+        const float d = sign * dp[u][r];
         p[u][r] = p0 - lam * p1;
-        part += p1 * dp[u][r];
-        s[0][u][r] = p0 * (dp[u][r] - st[2]);
-        s[1][u][r] = p1 * (dp[u][r] - st[3]);                                // -lam: at the end, once
+        part += p1 * d;
+        s[0][u][r] = p0 * (d - st[2]);
+        s[1][u][r] = p1 * (d - st[3]);                                       // -lam: at the end, once
       }
     dlam += part;
     frag_from(pf, p[0], p[1]);
