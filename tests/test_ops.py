@@ -535,6 +535,15 @@ def test_diff_attention_long_sweeps_of_few_heads(Tq, Tk, hd, t):
 
 
 @gpu
+@pytest.mark.parametrize("hd", [32, 64, 96, 128])
+@pytest.mark.parametrize("t", [BF, F32])
+@pytest.mark.parametrize("B,Tq,Tk,lens", [(24, 70, 70, None), (24, 161, 140, [140, 0, 17, 64, 133]), (96, 40, 33, [33, 1, 32])])
+def test_diff_attention_many_heads(B, Tq, Tk, lens, hd, t):
+    """Enough (sample, head) pairs to fill the card: the larger workgroups of every kernel."""
+    check_attention(B, Tq, Tk, 8, hd, t, lens=lens)
+
+
+@gpu
 @pytest.mark.parametrize("T", [20, 90])
 def test_diff_attention_nan_stays_in_its_sample(T):
     _, q, k, v, lam, n, g = attention_case(3, T, T, 2, 64, BF, None, False)
