@@ -30,6 +30,9 @@ struct Args {
   float *dq_part, *dk_part, *dv_part;
 };
 
+// A single row's stride may be anything; the kernels' tiles end where the row after it would begin
+inline int64_t row_step(int64_t ld, int T, int64_t w) { return T == 1 ? w : ld; }
+
 // Tq, Tk <= 32 (diffattn_short.hip); the backward needs dlam_part [H][B], no lse, out, out2 or delta
 constexpr int SHORT = 32;
 int short_attention(const Args& a, int dtype, int hd, bool backward, hipStream_t s);

@@ -341,7 +341,9 @@ int make_args(const gpt_diff_attention_t* p, const char* who, Args* a) {
               "%s: misaligned operand", who);
   *a = Args{};
   a->q = p->q; a->k = p->k; a->v = p->v;
-  a->ldq = p->ldq; a->bsq = p->bsq; a->ldk = p->ldk; a->bsk = p->bsk; a->ldv = p->ldv; a->bsv = p->bsv;
+  a->ldq = row_step(p->ldq, p->Tq, w); a->bsq = p->bsq;
+  a->ldk = row_step(p->ldk, p->Tk, w); a->bsk = p->bsk;
+  a->ldv = row_step(p->ldv, p->Tk, w); a->bsv = p->bsv;
   a->lam = p->lam; a->lengths = p->lengths;
   a->out = p->out; a->ldo = p->ldo; a->bso = p->bso; a->lse = p->lse; a->out2 = p->out2;
   a->B = p->B; a->Tq = p->Tq; a->Tk = p->Tk; a->H = p->n_head;

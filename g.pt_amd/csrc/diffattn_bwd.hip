@@ -606,7 +606,7 @@ extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_d
               "%s: gradient rows must be 16-byte aligned, a row's width or more apart", who);
   const int64_t need = bwd_workspace(f->dtype, f->B, f->Tq, f->Tk, f->n_head, f->hd);
   GPT_REQUIRE(p->ws && (uintptr_t)p->ws % 16 == 0 && p->ws_bytes >= need, "%s: needs %lld bytes of scratch", who, (long long)need);
-  a.dout = p->dout; a.lddo = p->lddo; a.bsdo = p->bsdo;
+  a.dout = p->dout; a.lddo = row_step(p->lddo, f->Tq, w); a.bsdo = p->bsdo;
   a.dq = p->dq; a.lddq = p->lddq; a.bsdq = p->bsdq;
   a.dk = p->dk; a.lddk = p->lddk; a.bsdk = p->bsdk;
   a.dv = p->dv; a.lddv = p->lddv; a.bsdv = p->bsdv;

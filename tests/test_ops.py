@@ -544,6 +544,34 @@ def test_diff_attention_many_heads(B, Tq, Tk, lens, hd, t):
 
 
 @gpu
+@pytest.mark.parametrize("t", [BF, F32])
+@pytest.mark.parametrize("Tq,Tk", [(1, 300), (40, 1), (1, 1)])
+def test_diff_attention_single_rows_may_have_any_stride_at_the_c_entry(Tq, Tk, t):
+    B, H, hd = 2, 2, 64
+    w, code = 2 * H * hd, L.BF16 if t == BF else L.F32
+    _, q, k, v, lam, _, g = attention_case(B, Tq, Tk, H, hd, t, None, False)
+    runs = []
+    for one in (w, 0, 32):                              # the stride of what has one row
+        ld = lambda T: one if T == 1 else w                                                                # noqa: E731,B023
+        out, out2, lse = torch.empty_like(q), torch.empty_like(q), torch.empty(2, B, H, Tq, device=DEV)
+        dq, dk, dv, dlam = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), torch.empty(H, device=DEV)
+        n = C.c_int64()
+        L.check(L.lib().gpt_diff_attention_workspace(code, B, Tq, Tk, H, hd, C.byref(n)), "workspace")
+        ws = torch.empty(max(16, n.value), dtype=torch.uint8, device=DEV)
+        f = L.DiffAttention(code, B, Tq, Tk, H, hd, hd ** -0.5, L.ptr(q), ld(Tq), Tq * w, L.ptr(k), ld(Tk), Tk * w, L.ptr(v), ld(Tk), Tk * w,
+                            L.ptr(lam), None, L.ptr(out), ld(Tq), Tq * w, L.ptr(lse), L.ptr(out2), L.ptr(ws), ws.numel())
+        L.check(L.lib().gpt_diff_attention(C.byref(f), L.stream()), "forward")
+        L.check(L.lib().gpt_diff_attention_bwd_workspace(code, B, Tq, Tk, H, hd, C.byref(n)), "workspace")
+        ws2 = torch.empty(max(16, n.value), dtype=torch.uint8, device=DEV)
+        b = L.DiffAttentionBwd(L.ptr(g), ld(Tq), Tq * w, L.ptr(dq), ld(Tq), Tq * w, L.ptr(dk), ld(Tk), Tk * w, L.ptr(dv), ld(Tk), Tk * w,
+                               L.ptr(dlam), L.ptr(ws2), ws2.numel())
+        L.check(L.lib().gpt_diff_attention_bwd(C.byref(f), C.byref(b), L.stream()), "backward")
+        runs.append([x.clone() for x in (out, dq, dk, dv, dlam)])
+    for other in runs[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(runs[0], other))
+
+
+@gpu
 @pytest.mark.parametrize("T", [20, 90])
 def test_diff_attention_nan_stays_in_its_sample(T):
     _, q, k, v, lam, n, g = attention_case(3, T, T, 2, 64, BF, None, False)
