@@ -519,7 +519,7 @@ struct DiffAttentionBackward : OnceNode {
       return res;
     }
     AttentionCall call(a);
-    const Tensor o = out.unpack(shared_from_this());
+    const Tensor o = kept ? out.unpack(shared_from_this()) : dq;         // not read where nothing was kept
     call.c.out = o.data_ptr(); call.c.ldo = o.stride(1); call.c.bso = o.stride(0);
     const Tensor lse_v = kept ? lse.unpack() : Tensor(), out2_v = kept ? out2.unpack() : Tensor();
     if (kept) { call.c.lse = lse_v.data_ptr<float>(); call.c.out2 = out2_v.data_ptr(); }
@@ -585,8 +585,7 @@ Tensor diff_attention_any(const char* who, const Tensor* qkv, const Tensor& q, c
     if (!qkv) { node->k = SavedVariable(k, false); node->v = SavedVariable(v, false); }
     node->lam = SavedVariable(a.lam, false);
     if (a.lengths.defined()) node->lengths = SavedVariable(a.lengths, false);
-    node->out = SavedVariable(o.out, true);
-    if (o.lse.defined()) { node->lse = SavedVariable(o.lse, false); node->out2 = SavedVariable(o.out2, false); }
+    if (node->kept) { node->out = SavedVariable(o.out, true); node->lse = SavedVariable(o.lse, false); node->out2 = SavedVariable(o.out2, false); }
   }
   return o.out;
 }

@@ -529,6 +529,9 @@ class Gpt(nn.Module):
         dec = self.decoder
         if not self.training or dec.dropout_p <= 0:
             return None
+        if torch.cuda.is_current_stream_capturing():
+            raise L.GptHipError("Gpt: dropout in a captured graph would repeat one step's masks at every replay; capture the model in "
+                                "evaluation mode or without dropout")
         seed = int(torch.randint(0, 2 ** 63 - 1, (), dtype=torch.int64))
         return L.DenoiserDropout(dec.embd_pdrop, dec.attn_pdrop, dec.resid_pdrop, seed, dp.get_rank() * (3 * dec.n_layer + 1), None)
 

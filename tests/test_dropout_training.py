@@ -203,6 +203,16 @@ def test_model_seeds_modes_and_no_grad(dtype):
     assert torch.equal(e, f) and torch.equal(state, torch.get_rng_state())
 
 
+def test_refuses_to_draw_masks_into_a_captured_graph(monkeypatch):
+    m = gpt_amd.Gpt(**dict(gpt_kwargs("mnist_small"), **PDROP)).train()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert isinstance(m.draw_dropout(), L.DenoiserDropout) and m.eval().draw_dropout() is None
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    assert m.draw_dropout() is None                      # evaluation mode: nothing to draw
+    with pytest.raises(L.GptHipError, match="captured graph"):
+        m.train().draw_dropout()
+
+
 @gpu
 @pytest.mark.parametrize("dtype,n_embd,n_head", [("fp32", 192, 2), ("bf16", 256, 4)])
 def test_train_step_uses_the_masks(dtype, n_embd, n_head):

@@ -572,6 +572,22 @@ def test_diff_attention_single_rows_may_have_any_stride_at_the_c_entry(Tq, Tk, t
 
 
 @gpu
+def test_diff_attention_output_changed_in_place():
+    """Up to 32 tokens the backward needs nothing of the forward's output, so it may be added to in place; longer ones notice."""
+    for T, kept in ((26, False), (60, True)):
+        _, q, k, v, lam, _, g = attention_case(2, T, T, 2, 64, BF, None, False)
+        leaves = [x.clone().requires_grad_() for x in (q, k, v, lam)]
+        want = torch.autograd.grad(ops.diff_attention(*leaves, 2), leaves, g)
+        out = ops.diff_attention(*leaves, 2)
+        out += 1
+        if kept:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(out, leaves, g)
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, g)))
+
+
+@gpu
 @pytest.mark.parametrize("T", [20, 90])
 def test_diff_attention_nan_stays_in_its_sample(T):
     _, q, k, v, lam, n, g = attention_case(3, T, T, 2, 64, BF, None, False)
