@@ -241,6 +241,15 @@ __device__ __forceinline__ f32x16 columns_product(const char* tile, const ColBas
   return acc;
 }
 
+// bf16: the 32 columns from chunk C of 16 rows of a tile as such a product's left operand; lo, hi: ColBase, moved to the rows
+template <int HD>
+__device__ __forceinline__ bf16x8 columns_frag(const char* tile, int lo, int hi, int C) {
+  using L = Tile<bf16_t, HD>;
+  const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(tile + L::add(lo, C)));
+  const v4s b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(tile + L::add(hi, C)));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // everything this wave has asked of memory and LDS is there, then everyone's is
 template <int LEFT>
 __device__ __forceinline__ void tile_barrier() {

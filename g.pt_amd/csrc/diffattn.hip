@@ -11,13 +11,15 @@
 // P enters the second product in the operands' type.  In bf16 that rounding adds as much noise as the output's own (out is off by
 // 2.5e-3 rms at 4096 keys, 1.7e-3 if only the output is rounded; the maps' difference cancels values, not their noise).  A second
 // operand with what the first rounding left takes it away: free where memory is the bound, so done there (one query group, <= 32
-// tokens); 4096 x 4096, hd 128, 32 (sample, head) would go from 441 to 616 us for it, 515 ragged, hd 64, from 60 to 77.
+// tokens); 4096 x 4096, hd 128, would go from 441 to 616 us for it, 515 ragged, hd 64, from 60 to 77.
 // The accumulator is rescaled only when a row's maximum has grown by more than a factor of 2^8 over the reference its sums are held
 // against: P stays below 2^8.
 #include "diffattn.h"
 
 namespace diffattn {
 namespace {
+
+#define PIN() __builtin_amdgcn_sched_barrier(0)
 
 constexpr float SLACK = 8.f;     // log2 of the growth that is let pass
 constexpr int MAX_SPLITS = 512;
@@ -31,6 +33,11 @@ template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   using L = Tile<T, HD>;
   constexpr int NT = NW * 128, KT = KEYS<T, NW>, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
+  // From hd 96 on, where two waves per SIMD are all the registers allow, the order is written out (PIN): operands read from LDS three
+  // matrix instructions ahead, the products of a tile's first 32 keys beside the exponentials of the other 32.  T = 4096, 16 (sample,
+  // head): hd 128 445 -> 406 us, hd 96 (half as many) 345 -> 330; hd 64, with three waves, 263 -> 271, hd 32 167 -> 161: left to the compiler
+  constexpr bool STEPPED = sizeof(T) == 2 && NW > 1 && HD >= 96;
+  constexpr int LEAD = 3, R = LEAD + 1;
   constexpr bool WHOLE = sizeof(T) == 2 && NW == 1;                       // P in two bf16 operands
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [2][K | V]
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
@@ -75,6 +82,22 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
     f32x16 s[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) s[u] = zero16();
+    if constexpr (STEPPED) {
+      int rk = rb + (it & 1) * 2 * TILE;                                     // opaque: the variants of it are formed as they are used
+      asm volatile("" : "+v"(rk));
+      constexpr int N = 2 * (L::CM / 2);
+      u32x4 ring[R];
+      auto rows = [&](int i) { return *reinterpret_cast<const u32x4*>(smem + (i & 1) * 32 * L::PITCH + L::add(rk, m * L::CM + (i & ~1))); };
+#pragma unroll
+      for (int i = 0; i < LEAD; ++i) ring[i] = rows(i);
+      PIN();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + LEAD < N) ring[(i + LEAD) % R] = rows(i + LEAD);
+        s[i & 1] = mma_chunk<T>(ring[i % R], qf[i / 2], s[i & 1]);
+        PIN();
+      }
+    } else
 #pragma unroll
     for (int c = 0; c < L::CM / 2; ++c)
 #pragma unroll
@@ -103,6 +126,42 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
     const float ref = top == -INFINITY ? 0.f : top * a.c2;                   // nothing but -inf so far: exp2(-inf) = 0
     float part = 0.f;                                                       // the tile's sum first: chains of 32 and of n additions, not 32 n
     Operand p[NU], low[WHOLE ? NU : 1];
+    if constexpr (STEPPED) {
+      int lo = cb.lo + (it & 1) * 2 * TILE + TILE, hi = cb.hi + (it & 1) * 2 * TILE + TILE;
+      asm volatile("" : "+v"(lo), "+v"(hi));
+      bf16x8 ring[R];
+      auto cols = [&](int u, int i) { return columns_frag<HD>(smem + (2 * u + (i & 1)) * 16 * L::PITCH, lo, hi, 4 * (i >> 1)); };
+      auto weigh = [&](int u, int e) {
+        s[u][e] = exp2_fast(s[u][e] * a.c2 - ref);
+        part += s[u][e];
+      };
+#pragma unroll
+      for (int i = 0; i < LEAD; ++i) ring[i] = cols(0, i);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) weigh(0, e);
+      operand_from<T>(p[0], s[0]);
+      PIN();
+      constexpr int N = 2 * CT;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {                                         // the first half's products beside the second half's weights
+#pragma unroll
+        for (int i = e * N / 16; i < (e + 1) * N / 16; ++i) {
+          ring[(i + LEAD) % R] = i + LEAD < N ? cols(0, i + LEAD) : cols(1, i + LEAD - N);
+          o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], p[0].p[i & 1], o[i >> 1], 0, 0, 0);
+        }
+        weigh(1, e);
+        if (e & 1) PIN();
+      }
+      operand_from<T>(p[1], s[1]);
+      sum += part;
+#pragma unroll
+      for (int i = N; i < 2 * N; ++i) {
+        if (i + LEAD < 2 * N) ring[(i + LEAD) % R] = cols(1, i + LEAD - N);
+        o[(i - N) >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], p[1].p[i & 1], o[(i - N) >> 1], 0, 0, 0);
+        PIN();
+      }
+      continue;
+    }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
