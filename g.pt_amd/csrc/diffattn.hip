@@ -35,7 +35,7 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   constexpr int NT = NW * 128, KT = KEYS<T, NW>, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
   // From hd 96 on, where two waves per SIMD are all the registers allow, the order is written out (PIN): operands read from LDS three
   // matrix instructions ahead, the products of a tile's first 32 keys beside the exponentials of the other 32.  T = 4096, 16 (sample,
-  // head): hd 128 445 -> 406 us, hd 96 (half as many) 345 -> 330; hd 64, with three waves, 263 -> 271, hd 32 167 -> 161: left to the compiler
+  // head): hd 128 445 -> 406 us, hd 96 345 -> 330; hd 64, with three waves, 263 -> 271, hd 32 167 -> 161: left to the compiler
   constexpr bool STEPPED = sizeof(T) == 2 && NW > 1 && HD >= 96;
   constexpr int LEAD = 3, R = LEAD + 1;
   constexpr bool WHOLE = sizeof(T) == 2 && NW == 1;                       // P in two bf16 operands

@@ -448,13 +448,29 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
   }
 }
 
+// dlam[h] = -(sum of the head's partial sums): a workgroup, each thread every 256th in index order, then a fixed tree
+__device__ __forceinline__ void sum_dlam(const float* __restrict__ part, int64_t n, int h, float* __restrict__ dlam) {
+  __shared__ float red[4];
+  const float* p = part + (int64_t)h * n;
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 256) s += p[i];
+  s = wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) dlam[h] = -((red[0] + red[1]) + (red[2] + red[3]));
+}
+__global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ part, int64_t n, float* __restrict__ dlam) {
+  sum_dlam(part, n, blockIdx.x, dlam);
+}
+
 // the spans' sums of dQ (where the keys were split) and of dK, dV (where the queries were), added in the spans' order: a thread owns 4
-// columns of a row
+// columns of a row.  The first n_head workgroups sum dlam instead
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void join_kernel(Args a) {
+__global__ __launch_bounds__(256) void join_kernel(Args a, int64_t parts, float* dlam) {
   constexpr int W = 2 * HD, PER = W / 4;
   const int64_t pairs = (int64_t)a.B * a.H, nq = a.k_splits > 1 ? pairs * a.Tq : 0, nk = a.q_splits > 1 ? pairs * a.Tk : 0;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if ((int)blockIdx.x < a.H) return sum_dlam(a.dlam_part, parts, blockIdx.x, dlam);
+  const int64_t i = (int64_t)(blockIdx.x - a.H) * 256 + threadIdx.x;
   int64_t row = i / PER;
   const int c = (int)(i - row * PER) * 4;
   if (row >= nq + 2 * nk) return;
@@ -469,18 +485,6 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   const int64_t b = pair / a.H, h = pair - b * a.H;
   T* out = (T*)(is_q ? a.dq : is_k ? a.dk : a.dv) + b * (is_q ? a.bsdq : is_k ? a.bsdk : a.bsdv) + t * (is_q ? a.lddq : is_k ? a.lddk : a.lddv);
   store4(out + h * W + c, sum);
-}
-
-// dlam[h] = -(sum of the head's partial sums): one workgroup per head, each thread every 256th in index order, then a fixed tree
-__global__ __launch_bounds__(256) void dlam_kernel(const float* __restrict__ part, int64_t n, float* __restrict__ dlam) {
-  __shared__ float red[4];
-  const float* p = part + (int64_t)blockIdx.x * n;
-  float s = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += 256) s += p[i];
-  s = wave_sum(s);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) dlam[blockIdx.x] = -((red[0] + red[1]) + (red[2] + red[3]));
 }
 
 // waves of 16 rows per workgroup: eight share the tiles where that still gives every CU a workgroup; fp32 from hd 96 on: four, which may
@@ -561,14 +565,13 @@ int launch(const Args& a, const Plan& plan, f32x4* stats, float* dlam, hipStream
   constexpr int M = MANY<T, HD>, MK = MANY_KEYS<T, HD>;
   if (int st = plan.many_k ? launch_dkv<T, HD, MK>(a, s) : launch_dkv<T, HD, FEW>(a, s)) return st;
   if (int st = plan.many_q ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, FEW>(a, s)) return st;
-  const int64_t joined = ((a.k_splits > 1 ? rows : 0) + (a.q_splits > 1 ? 2 * pairs * a.Tk : 0)) * (HD / 2);
-  if (joined > 0) {
-    hipLaunchKernelGGL((join_kernel<T, HD>), dim3((unsigned)((joined + 255) / 256)), dim3(256), 0, s, a);
-    if (int st = gpt_launch_status(who)) return st;
-  }
   const int nk = plan.many_k ? MK : FEW;
   const int64_t parts = (int64_t)a.B * a.q_splits * (((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk);
-  hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, parts, dlam);
+  const int64_t joined = ((a.k_splits > 1 ? rows : 0) + (a.q_splits > 1 ? 2 * pairs * a.Tk : 0)) * (HD / 2);
+  if (joined > 0)
+    hipLaunchKernelGGL((join_kernel<T, HD>), dim3((unsigned)(a.H + (joined + 255) / 256)), dim3(256), 0, s, a, parts, dlam);
+  else
+    hipLaunchKernelGGL(dlam_kernel, dim3(a.H), dim3(256), 0, s, a.dlam_part, parts, dlam);
   return gpt_launch_status(who);
 }
 
