@@ -1,4 +1,5 @@
-// What the differential-attention kernels share: the launch's arguments, 16 x 16 matrix-core tiles of both types, masks.
+// What the differential-attention kernels share: the launch's arguments, tiles in LDS and their loads, 32 x 32 matrix products of both
+// types.
 #pragma once
 #include "common.h"
 

@@ -9,7 +9,9 @@
 // D_i = sum P_i dP are sums over a lane's registers and one exchange, in fp32 throughout.  The backward takes both transposed uses
 // (dQ contracts over keys, dK and dV over queries) from one evaluation: dS_i^T is dQ's operand as it stands in the registers; dS_i
 // and P go once through LDS for the other two.
-// HBM-bound: the backward moves 11 row sets of Tq or Tk x 2 hd for some 2 MFLOP each.
+// HBM-bound: the backward moves 11 row sets of Tq or Tk x 2 hd for some 2 MFLOP each, the forward 4 (it feeds the maps' difference as
+// two bf16 operands, 16 bits, at no cost).  1024 samples x 26 tokens, 8 heads of 2 x 96, bf16: forward 74 us (64 at a copy's rate),
+// backward 124 (111); 64 samples forward 7.6.
 #include "short_tiles.h"
 
 namespace diffattn {
