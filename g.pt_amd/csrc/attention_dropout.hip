@@ -1,5 +1,5 @@
 // Multi-head attention over T <= 32 tokens with dropout on its probabilities, forward and backward: what attention.hip computes, for a
-// training step with attn_pdrop > 0 (Gpt/models/transformer.py:43-47, the Dropout of :27).
+// training step with attn_pdrop > 0 (Gpt/models/transformer.py:34-51).
 //
 //   P = softmax(q k^T / sqrt(hd)),   P~ = keep * s * P,   y = P~ v
 //   dP = keep * s * (dy v^T),   D = sum_j P dP,   dS = P (dP - D),   dq = dS k / sqrt(hd),   dk = dS^T q / sqrt(hd),   dv = P~^T dy

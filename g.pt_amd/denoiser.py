@@ -524,7 +524,7 @@ class Gpt(nn.Module):
         return x, t, lt, lp, x_prev
 
     def draw_dropout(self):
-        """The dropout masks of one forward in training mode (transformer.py:27-28, 66, 219): probabilities, and a seed drawn from
+        """The dropout masks of one forward in training mode (transformer.py:34-72, 302-314): probabilities, and a seed drawn from
         torch's CPU generator, so torch.manual_seed makes runs repeatable; every rank takes offsets of its own.  None without dropout."""
         dec = self.decoder
         if not self.training or dec.dropout_p <= 0:

@@ -525,7 +525,7 @@ typedef struct {
 } gpt_dropout_t;
 
 /* out[r, c] (x_dtype) = (resid ? resid[r, c] (x_dtype) : 0) + (kept ? h[r, c] (h_dtype) * 65536 / (65536 - thr) : 0).
- * Replaces nn.Dropout and the residual addition behind it (Gpt/models/transformer.py:27-28, 50, 66, 70-71).  The gradient of h is
+ * Replaces nn.Dropout and the residual addition behind it (Gpt/models/transformer.py:34-72).  The gradient of h is
  * this call on the gradient of out with the same `drop` and resid = NULL; that of resid is the gradient of out itself.
  * ldh / ldr / ldo: elements from row to row (inputs may have 0); any alignment of whole elements (rows of 16-byte aligned
  * multiples of 8 elements, or contiguous tensors, take the vector path).  out may be resid or h (same type, same strides).
@@ -632,7 +632,7 @@ int gpt_attention_dropout(int dtype, const void* qkv, void* y, int B, int T, int
 int gpt_attention_dropout_bwd(int dtype, const void* qkv, const void* dy, void* dqkv, int B, int T, int n_head, int hd,
                               const gpt_dropout_t* drop, void* stream);
 
-/* The probabilities of transformer.py:27-28, 66, 219 (embd: position-embedded tokens; attn: attention probabilities; resid: the
+/* The probabilities of transformer.py:34-72, 302-314 (embd: position-embedded tokens; attn: attention probabilities; resid: the
  * outputs of both residual branches of a Block).  The masks of a step take the offsets offset .. offset + 3 n_layer: site 0 = embd,
  * 1 + 3 l, 2 + 3 l, 3 + 3 l = Block l's attention, projection and MLP; forward and backward of a step are given the same struct.
  * (Where the last Block works on the decoded tokens' rows alone, its two residual masks are those of the compact rows.) */

@@ -1,4 +1,4 @@
-"""Dropout in the denoiser's training path (transformer.py:27-28, 45, 50, 66, 219): attention with dropped-out probabilities against
+"""Dropout in the denoiser's training path (transformer.py:34-72, 302-314): attention with dropped-out probabilities against
 its formula in 64 bits, and the whole model, forward and gradients, against a 64-bit restatement that applies the same masks."""
 import ctypes as C
 import math
