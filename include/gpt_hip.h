@@ -625,7 +625,7 @@ int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk, int n_hea
 int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_diff_attention_bwd_t* g, void* stream);
 
 /* ---- dropout in the denoiser's training step ------------------------------------------------------------------------------------
- * gpt_attention_rows with dropout on the softmax probabilities (Gpt/models/transformer.py:45-46), and its backward (dqkv is stored):
+ * gpt_attention_rows with dropout on the softmax probabilities (Gpt/models/transformer.py:43-47), and its backward (dqkv is stored):
  * element (((sample * n_head + head) * T + query) * 32 + key) of the mask.  T <= 32, hd 32, 64, 96 or 128. */
 int gpt_attention_dropout(int dtype, const void* qkv, void* y, int B, int T, int t_out, int n_head, int hd, const gpt_dropout_t* drop,
                           void* stream);

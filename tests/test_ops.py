@@ -35,11 +35,11 @@ def within(got, want, tol, what=""):
 
 
 # ---------------------------------------------------------------------------------------------------------------- dropout
-def philox_keep(n, p, seed, offset):
-    """Keep mask of elements 0 .. n - 1 from the published Philox4x32-10 (unsigned 64-bit words on the host)."""
+def philox_keep(n, p, seed, offset, first=0):
+    """Keep mask of elements first .. first + n - 1 (8 | first) from the published Philox4x32-10 (unsigned 64-bit words on the host)."""
     u = np.uint64
     m, s32 = u(0xFFFFFFFF), u(32)
-    blk = np.arange((n + 7) // 8, dtype=u)
+    blk = np.arange(first // 8, first // 8 + (n + 7) // 8, dtype=u)
     c = [blk & m, blk >> s32, np.full_like(blk, offset & 0xFFFFFFFF), np.full_like(blk, offset >> 32)]
     k0, k1 = seed & 0xFFFFFFFF, seed >> 32
     for _ in range(10):
@@ -162,6 +162,18 @@ def test_dropout_counter_and_graph_replay():
     counter.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         x.sum().backward()
+
+
+@gpu
+def test_dropout_beyond_32_bits_of_elements():
+    rows, d, last = (1 << 20) + 3, 4104, 5 * 4104
+    h = torch.ones(rows, d, dtype=BF, device=DEV)
+    y = ops.dropout(h, 0.5, 77, 5)
+    n = rows * d
+    assert n > 1 << 32
+    for first in (0, (1 << 32) - last // 2 // 8 * 8, n - last):
+        want = philox_keep(last, 0.5, 77, 5, first).to(BF) * 2
+        assert torch.equal(y.view(-1)[first:first + last].cpu(), want), first
 
 
 @gpu
@@ -585,6 +597,24 @@ def test_diff_attention_output_changed_in_place():
                 torch.autograd.grad(out, leaves, g)
         else:
             assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, g)))
+
+
+@gpu
+@pytest.mark.parametrize("Tq", [1, 40])
+def test_diff_attention_rows_beyond_32_bits(Tq):
+    """A long cache whose rows lie 512 KiB apart: offsets pass 2^32 bytes, forward and backward, as in a compact cache."""
+    Tk, w = 9000, 64
+    cache = torch.empty(Tk, 1 << 18, dtype=BF, device=DEV)
+    cache[:, :2 * w] = normal(1, Tk, 2 * w, dtype=BF)
+    q, lam, g = normal(2, 1, Tq, w, dtype=BF), torch.tensor([0.4], device=DEV), normal(3, 1, Tq, w, dtype=BF)
+    runs = []
+    for compact in (False, True):
+        k, v = (cache[None, :, i * w:(i + 1) * w] for i in (0, 1))
+        leaves = [x.detach().requires_grad_() for x in ((q, k.contiguous(), v.contiguous(), lam) if compact else (q, k, v, lam))]
+        assert leaves[1].stride(1) == (w if compact else 1 << 18)
+        out = ops.diff_attention(*leaves, 1)
+        runs.append((out.detach(), *torch.autograd.grad(out, leaves, g)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
 
 
 @gpu
