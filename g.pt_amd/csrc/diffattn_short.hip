@@ -9,9 +9,11 @@
 // D_i = sum P_i dP are sums over a lane's registers and one exchange, in fp32 throughout.  The backward takes both transposed uses
 // (dQ contracts over keys, dK and dV over queries) from one evaluation: dS_i^T is dQ's operand as it stands in the registers; dS_i
 // and P go once through LDS for the other two.
-// HBM-bound: the backward moves 11 row sets of Tq or Tk x 2 hd for some 2 MFLOP each, the forward 4 (it feeds the maps' difference as
-// two bf16 operands, 16 bits, at no cost).  1024 samples x 26 tokens, 8 heads of 2 x 96, bf16: forward 74 us (64 at a copy's rate),
-// backward 124 (111); 64 samples forward 7.6.
+// bf16: P and dS enter their products as two operands each (16 bits of mantissa; the values are exact products of them), so the
+// results' own rounding is the only one to 8 bits.  HBM-bound, which is why that costs little: the backward reads 4 row sets of Tq or
+// Tk x 2 hd and writes 3 for some 2 MFLOP each, the forward 3 and 1.  1024 samples x 26 tokens, 8 heads of 2 x 96, bf16: forward
+// 74 us (64 at a copy's rate), backward 130 (111; 124 with one operand, whose dQ, dK, dV are off by 2.35e-3 rms instead of
+// 1.66e-3); 64 samples forward 7.6.
 #include "short_tiles.h"
 
 namespace diffattn {
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 3 : 1) void short_fwd_kernel(A
 template <typename T, int HD>
 __global__ __launch_bounds__(64, sizeof(T) == 2 && HD < 128 ? 2 : 1) void short_bwd_kernel(Args a) {
   using L = Tile<T, HD>;
-  constexpr int NT = 2 * HD / 32, HALF = NT / 2;
+  constexpr int NT = 2 * HD / 32, HALF = NT / 2, PARTS = sizeof(T) == 2 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x, r = lane & 31, hh = lane >> 5;
   const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, len = valid_keys(a, b);
@@ -117,18 +119,29 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 && HD < 128 ? 2 : 1) void short_
     s[0][e] = in ? s[0][e] * (dp[e] - d[0]) : 0.f;
     s[1][e] = in ? -lam * (s[1][e] * (dp[e] - d[1])) : 0.f;
   }
-  // dS_i^T is dQ's operand as it stands; P, dS_1 and dS_2 go through the one matrix buffer in turn
-  Operand x, xp, xs[2];
-  if (qok) put_matrix<T>(tm, p, r, hh);
-  lds_done();
-  get_matrix<T>(xp, tm, a.Tq, lane, zero);
+  // dS_i^T is dQ's operand as it stands; P, dS_1 and dS_2 go through the one matrix buffer in turn, in bf16 each as two operands
+  Operand x, low, xp[2], xs[2][2];
+  auto turn = [&](Operand (&o)[2], f32x16 m) {
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    lds_done();
-    if (qok) put_matrix<T>(tm, s[m], r, hh);
-    lds_done();
-    get_matrix<T>(xs[m], tm, a.Tq, lane, zero);
-  }
+    for (int part = 0; part < PARTS; ++part) {
+      lds_done();
+      if (qok) put_matrix<T>(tm, m, r, hh);
+      lds_done();
+      get_matrix<T>(o[part], tm, a.Tq, lane, zero);
+      if constexpr (PARTS == 2)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m[e] -= bf16_to_f32(f32_to_bf16(m[e]));   // what put_matrix's rounding leaves
+    }
+  };
+  turn(xp, p);
+#pragma unroll
+  for (int m = 0; m < 2; ++m) turn(xs[m], s[m]);
+  auto product = [&](auto order, const char* tile, int n, int t, const Operand& hi, const Operand& lo) {
+    if constexpr (PARTS == 2) return columns_product<T, L, order.value>(tile, n, t, hi, lane, zero, lo);
+    else return columns_product<T, L, order.value>(tile, n, t, hi, lane, zero);
+  };
+  constexpr std::integral_constant<int, 0> by_key{};
+  constexpr std::integral_constant<int, 1> by_query{};
   // each output leaves through the tile of the operand that its products have just read (all tiles have max(Tq, Tk) rows)
   f32x16 acc[NT];
   auto put = [&](char* tile, T* dst, int64_t ld, int n, float scale) {
@@ -142,15 +155,16 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 && HD < 128 ? 2 : 1) void short_
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     operand_from<T>(x, s[m]);
+    if constexpr (PARTS == 2) operand_rest(low, s[m], x);
 #pragma unroll
-    for (int t = m * HALF; t < (m + 1) * HALF; ++t) acc[t] = columns_product<T, L, 0>(tk, a.Tk, t, x, lane, zero);       // dQ_m^T = K_m^T dS_m^T
+    for (int t = m * HALF; t < (m + 1) * HALF; ++t) acc[t] = product(by_key, tk, a.Tk, t, x, low);                          // dQ_m^T = K_m^T dS_m^T
   }
   put(tk, (T*)a.dq + (int64_t)b * a.bsdq + h * 2 * HD, a.lddq, a.Tq, a.scale);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = columns_product<T, L, 1>(tq, a.Tq, t, xs[t / HALF], lane, zero);                 // dK_m^T = Q_m^T dS_m
+  for (int t = 0; t < NT; ++t) acc[t] = product(by_query, tq, a.Tq, t, xs[t / HALF][0], xs[t / HALF][PARTS - 1]);        // dK_m^T = Q_m^T dS_m
   put(tq, (T*)a.dk + (int64_t)b * a.bsdk + h * 2 * HD, a.lddk, a.Tk, a.scale);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) acc[t] = columns_product<T, L, 1>(tg, a.Tq, t, xp, lane, zero);                           // dV^T = dO^T P
+  for (int t = 0; t < NT; ++t) acc[t] = product(by_query, tg, a.Tq, t, xp[0], xp[PARTS - 1]);                            // dV^T = dO^T P
   put(tg, (T*)a.dv + (int64_t)b * a.bsdv + h * 2 * HD, a.lddv, a.Tk, 1.f);
 }
 
