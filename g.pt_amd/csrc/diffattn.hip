@@ -8,10 +8,11 @@
 // A wave takes 32 queries and ONE map: its accumulator is 32 x 2 hd (128 registers at hd 128) where both maps' would leave one wave
 // per SIMD; the two waves of a query group join their halves through LDS at the end.  K | V tiles of 64 or 32 keys come by
 // LDS-DMA, double-buffered, one barrier per tile, and serve all waves of the workgroup.
-// P enters the second product in the operands' type.  In bf16 that rounding adds as much noise as the output's own (out is off by
-// 2.5e-3 rms at 4096 keys, 1.7e-3 if only the output is rounded; the maps' difference cancels values, not their noise).  A second
-// operand with what the first rounding left takes it away: free where memory is the bound, so done there (one query group, <= 32
-// tokens); 4096 x 4096, hd 128, would go from 441 to 616 us for it, 515 ragged, hd 64, from 60 to 77.
+// bf16: P enters the second product as two operands, its rounding to bf16 and what that left (16 bits of mantissa), so that the output's
+// own rounding is the only one to 8 bits.  One operand alone leaves the output 2.55e-3 rms off at 4096 keys where rounding the exact
+// result leaves 1.66e-3 (the maps' difference cancels values, not their noise).  The second costs nothing where memory is the bound (one
+// query group) and, where the matrix unit is, half of its work again: 2 x 4096 tokens, 8 heads, hd 128, 560 us (1.23 PFLOP/s of its 687
+// GFLOP) instead of 406, 16 samples of up to 515 tokens, hd 64, 50 instead of 44.
 // The accumulator is rescaled only when a row's maximum has grown by more than a factor of 2^8 over the reference its sums are held
 // against: P stays below 2^8.
 #include "diffattn.h"
@@ -33,12 +34,12 @@ template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   using L = Tile<T, HD>;
   constexpr int NT = NW * 128, KT = KEYS<T, NW>, NU = KT / 32, TILE = KT * L::PITCH, CT = 2 * HD / 32;
-  // From hd 96 on, where two waves per SIMD are all the registers allow, the order is written out (PIN): operands read from LDS three
-  // matrix instructions ahead, the products of a tile's first 32 keys beside the exponentials of the other 32.  T = 4096, 16 (sample,
-  // head): hd 128 445 -> 406 us, hd 96 345 -> 330; hd 64, with three waves, 263 -> 271, hd 32 167 -> 161: left to the compiler
-  constexpr bool STEPPED = sizeof(T) == 2 && NW > 1 && HD >= 96;
+  // From hd 64 on the order is written out (PIN): operands read from LDS three fragments ahead, the products of a tile's first 32 keys
+  // beside the exponentials of the other 32.  2 x 4096 tokens, 8 heads: hd 128 617 -> 584 us, hd 96 490 -> 471, hd 64 370 -> 351; hd 32
+  // 216 -> 218: left to the compiler
+  constexpr bool STEPPED = sizeof(T) == 2 && NW > 1 && HD >= 64;
   constexpr int LEAD = 3, R = LEAD + 1;
-  constexpr bool WHOLE = sizeof(T) == 2 && NW == 1;                       // P in two bf16 operands
+  constexpr bool WHOLE = sizeof(T) == 2;                                  // P in two bf16 operands
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [2][K | V]
   const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, hh = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), m = wid & 1, grp = wid >> 1;
@@ -140,6 +141,7 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) weigh(0, e);
       operand_from<T>(p[0], s[0]);
+      operand_rest(low[0], s[0], p[0]);
       PIN();
       constexpr int N = 2 * CT;
 #pragma unroll
@@ -148,16 +150,19 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
         for (int i = e * N / 16; i < (e + 1) * N / 16; ++i) {
           ring[(i + LEAD) % R] = i + LEAD < N ? cols(0, i + LEAD) : cols(1, i + LEAD - N);
           o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], p[0].p[i & 1], o[i >> 1], 0, 0, 0);
+          o[i >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], low[0].p[i & 1], o[i >> 1], 0, 0, 0);
         }
         weigh(1, e);
         if (e & 1) PIN();
       }
       operand_from<T>(p[1], s[1]);
+      operand_rest(low[1], s[1], p[1]);
       sum += part;
 #pragma unroll
       for (int i = N; i < 2 * N; ++i) {
         if (i + LEAD < 2 * N) ring[(i + LEAD) % R] = cols(1, i + LEAD - N);
         o[(i - N) >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], p[1].p[i & 1], o[(i - N) >> 1], 0, 0, 0);
+        o[(i - N) >> 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[i % R], low[1].p[i & 1], o[(i - N) >> 1], 0, 0, 0);
         PIN();
       }
       continue;

@@ -6,10 +6,13 @@
 // order); dlam is summed from the fp32 P_2 and dP of the second sweep (from the rounded outputs it would carry their rounding error).
 // A wave holds 16 rows of its side for BOTH maps - operands and accumulators, some 230 registers at hd 128, two waves per SIMD: dP
 // serves both maps, so a wave per map would compute it twice (a third more matrix work in dQ, a half in dK / dV), and 32 rows per wave
-// would leave one wave per SIMD with nothing beside it while it waits for LDS or exponentials (T = 4096, 16 (sample, head), hd 128: dK
-// / dV 1069 us, dQ 735; as it is 640 and 470, 860 and 880 TFLOP/s of their own work. The matrix instructions alone take 417 of the
-// 640, at the clock that the chip's power leaves them). The other side comes in tiles of 32 rows by LDS-DMA, shared by the
-// workgroup's waves; every tile is used twice, by rows for the scores and transposed for the gradient products.
+// would leave one wave per SIMD with nothing beside it while it waits for LDS or exponentials (T = 4096, 16 (sample, head), hd 128, with
+// one bf16 operand: dK / dV 1069 us, dQ 735; with 16 rows 640 and 470).  The other side comes in tiles of 32 rows by LDS-DMA, shared
+// by the workgroup's waves; every tile is used twice, by rows for the scores and transposed for the gradient products.
+// bf16: P and dS enter the gradient products as two operands each (16 bits of mantissa), so that the gradients' own rounding is the
+// only one to 8 bits: one operand leaves dQ, dK, dV 2.35e-3 rms off where rounding the exact result leaves 1.66e-3.  It costs half of
+// dK / dV's matrix work again and a third of dQ's: 737 and 521 us (1.12 and 1.06 PFLOP/s of their 824 and 550 GFLOP) instead of 640 and
+// 470; 16 samples of up to 515 tokens, hd 64, 57 and 46 instead of 47 and 39.
 #include "diffattn.h"
 
 namespace diffattn {
@@ -64,12 +67,21 @@ __device__ __forceinline__ Frag<float> frag_row(const float* p, int c, int g, bo
   }
   return f;
 }
-// two accumulator tiles (rows 0..15 and 16..31 of the contraction) as an operand; bf16: rounded once
-__device__ __forceinline__ void frag_from(Frag<bf16_t>& f, const f32x4& lo, const f32x4& hi) {
-  const uint32_t w[4] = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
-  f.v = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+// two accumulator tiles (rows 0..15 and 16..31 of the contraction) as an operand; bf16: as two, `low` what the rounding to the first
+// leaves (16 bits of mantissa together; fp32 has no second)
+__device__ __forceinline__ void frag_pair(Frag<bf16_t>& f, Frag<bf16_t>& low, const f32x4& lo, const f32x4& hi) {
+#pragma clang fp contract(off)                                           // (an fma with the product that x is would keep both its factors)
+  u32x4 w, v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = j < 2 ? lo[2 * j] : hi[2 * j - 4], y = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
+    w[j] = pack_bf16x2(x, y);
+    v[j] = pack_bf16x2(x - __uint_as_float(w[j] << 16), y - __uint_as_float(w[j] & 0xffff0000u));
+  }
+  f.v = __builtin_bit_cast(bf16x8, w);
+  low.v = __builtin_bit_cast(bf16x8, v);
 }
-__device__ __forceinline__ void frag_from(Frag<float>& f, const f32x4& lo, const f32x4& hi) {
+__device__ __forceinline__ void frag_pair(Frag<float>& f, Frag<float>&, const f32x4& lo, const f32x4& hi) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     f.v[j] = lo[j];
@@ -182,6 +194,12 @@ constexpr int STAGES = sizeof(T) == 2 && NW == 8 ? 3 : 2;
 // use and waits out the LDS latency there (dK / dV at T = 4096, hd 128: 850 us).  PIN() keeps the written order.
 template <typename T>
 constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
+// x, opaque to the compiler: what is formed from it is formed where it is used and holds no register over the loop
+template <typename V>
+__device__ __forceinline__ V opaque(V x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 #define PIN() __builtin_amdgcn_sched_barrier(0)
 
 // dQ: NW waves of 16 queries; K | V tiles of 32 keys.  S_i^T = K_i Q_i^T and dP^T = V dO^T: keys on the accumulator's rows.
@@ -231,7 +249,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
   constexpr int NA = 4 * KC, R = AHEAD<T> + 1;
   const bool late = NS == 3 && wid >= NW / 2;
   f32x4 dp[2], s[2][2];
-  Frag<T> ring[R], x[2];
+  Frag<T> ring[R], x[2], low[2];
   auto scores = [&](int at, int it) {
     // the lane's place in this stage, opaque to the compiler: it would keep every variant of it in a register over the loop
     int rk = rb + at;
@@ -269,8 +287,8 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
           for (int r = 0; r < 4; ++r)
             if (it * 32 + 16 * u + 4 * g + r >= len) s[m][u][r] = 0.f;
     }
-    frag_from(x[0], s[0][0], s[0][1]);
-    frag_from(x[1], s[1][0], s[1][1]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) frag_pair(x[m], low[m], s[m][0], s[m][1]);
   };
   auto products = [&](int at) {
     int ck = cb + at;
@@ -282,6 +300,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     for (int t = 0; t < 2 * CT; ++t) {
       if (t + AHEAD<T> < 2 * CT) ring[(t + AHEAD<T>) % R] = col16<T, HD>(smem, ck, t + AHEAD<T>);
       acc[t] = mma16(ring[t % R], x[t / CT], acc[t]);
+      if constexpr (sizeof(T) == 2) acc[t] = mma16(ring[t % R], low[t / CT], acc[t]);
       PIN();
     }
   };
@@ -310,7 +329,7 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
 // dK, dV and the tile's share of sum P_2 dP: NW waves of 16 keys; Q | dO | statistics tiles of 32 queries.  S_i = Q_i K_i^T and
 // dP = dO V^T: queries on the accumulator's rows.  Queries behind Tq arrive as zeros in all three: their dP, D and products are 0.
 template <typename T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HD == 64 ? 3 : 1) void dkv_kernel(Args a) {
   using L = Tile<T, HD>;
   constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, STAGE = 2 * TILE + 512, KC = HD / 32, CT = HD / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [NS][Q | dO | stats]
@@ -356,16 +375,14 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
     dma_tile<T, HD, 32, NT>(gb + (int64_t)it * 32 * a.lddo, a.lddo, a.Tq - it * 32, dst + TILE, tid, wid);
     if (wid == 0) dma_bytes(sb + it * 32, (a.Tq - it * 32) * 16, dst + 2 * TILE, lane);
   };
-  constexpr int NA = 4 * KC, LEAD = HD == 128 && sizeof(T) == 2 ? 2 : AHEAD<T>, R = LEAD + 1;   // (3 at hd 128: over 256 registers)
+  constexpr int NA = 4 * KC, LEAD = HD == 128 && sizeof(T) == 2 ? 2 : AHEAD<T>, R = LEAD + 1;   // (3 at hd 128: 251 registers and no faster)
   const bool late = NS == 3 && wid >= NW / 2;                               // as in dq_kernel
   f32x4 dp[2], p[2], s[2][2];
-  Frag<T> ring[R], pf, df[2];
+  Frag<T> ring[R], pf, df[2], pl, dl[2];
   auto scores = [&](int at) {
-    int rq = rb + at, sq = 64 * g + at;
-    asm volatile("" : "+v"(rq), "+v"(sq));
-    const f32x4* ts = reinterpret_cast<const f32x4*>(smem + 2 * TILE + sq);
+    int rq = rb + at;
+    asm volatile("" : "+v"(rq));
     auto rows = [&](int u, int i) { return row16<T, HD>(smem + (i & 1 ? 0 : TILE), rq, 16 * u, i / 2); };
-    float part = 0.f;
 #pragma unroll
     for (int i = 0; i < LEAD; ++i) ring[i] = rows(0, i);
     PIN();
@@ -382,6 +399,8 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         PIN();
       }
     }
+    float part = 0.f;
+    const f32x4* ts = reinterpret_cast<const f32x4*>(smem + 2 * TILE + 64 * (opaque(lane) >> 4) + at);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -394,10 +413,10 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
         s[0][u][r] = p0 * (d - st[2]);
         s[1][u][r] = p1 * (d - st[3]);                                       // -lam: at the end, once
       }
-    dlam += part;
-    frag_from(pf, p[0], p[1]);
-    frag_from(df[0], s[0][0], s[0][1]);
-    frag_from(df[1], s[1][0], s[1][1]);
+    dlam += opaque(part);                                                    // here, not behind the products: its terms would be kept over them
+    frag_pair(pf, pl, p[0], p[1]);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) frag_pair(df[m], dl[m], s[m][0], s[m][1]);
   };
   auto products = [&](int at) {
     int cq = cb + at;
@@ -412,6 +431,10 @@ __global__ __launch_bounds__(NW * 64) void dkv_kernel(Args a) {
       if (i + LEAD < 4 * CT) ring[(i + LEAD) % R] = cols(i + LEAD);
       if (i & 1) dk[t] = mma16(ring[i % R], df[t / CT], dk[t]);
       else dv[t] = mma16(ring[i % R], pf, dv[t]);
+      if constexpr (sizeof(T) == 2) {
+        if (i & 1) dk[t] = mma16(ring[i % R], dl[t / CT], dk[t]);
+        else dv[t] = mma16(ring[i % R], pl, dv[t]);
+      }
       PIN();
     }
   };
@@ -492,19 +515,20 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, int64_t parts, float*
 // have 512 registers each (eight would spill)
 template <typename T, int HD>
 constexpr int MANY = sizeof(T) == 4 && HD >= 96 ? 4 : 8;
-// dK / dV in bf16 at hd 64: 170 registers, so three waves per SIMD in workgroups of four, two in workgroups of eight (4 x 4096 tokens,
-// 8 heads: 787 and 835 us; 16 samples of up to 515: 58 and 65.  At hd 32, 4 x 4096: 490 and 459; hd 128, T = 4096: 1034 and 636)
+// dK / dV in bf16 at hd 64: three waves per SIMD in workgroups of four, which the launch bounds ask for (unasked it took 176 registers:
+// 16 samples of up to 515 tokens 67 us, now 57), two in workgroups of eight (4 x 4096 tokens, 8 heads: 870 and 930 us; 16 x 515: 93 and
+// 115.  At hd 32, 4 x 4096: 656 and 591; hd 128, T = 4096: 1092 and 760)
 template <typename T, int HD>
 constexpr int MANY_KEYS = sizeof(T) == 2 && HD == 64 ? 4 : MANY<T, HD>;
 // ... else four, one per SIMD: two workgroups of two waves share SIMDs while others idle (32 (sample, head) x 512 tokens, hd 128: dK / dV
-// and dQ 47 and 42 us in bf16, 43 and 31 by fours; in fp32 180 and 226, 168 and 126)
+// and dQ 51 and 48 us in bf16, 45 and 34 by fours; in fp32 180 and 226, 168 and 126)
 constexpr int FEW = 4;
 bool many_waves(int64_t pairs, int T) { return T > 32 && pairs * ((T + 127) / 128) >= 192; }
 
 // How a call is cut.  Workgroups of four waves that do not fill the CUs have their sweep split into spans, up to one workgroup per CU
 // (two where registers and LDS leave room: hd <= 64), whose sums are joined by a launch of their own (6 to 10 us): worth it from 5
 // tiles of 32 rows per span in bf16 and, the matrix rate being an eighth there, from 2 in fp32.  dK / dV and dQ, unsplit and split:
-// 16 (sample, head) x 257 tokens, hd 96, fp32: 67 and 52 us, 32 and 24; 2 x 2048, hd 128, bf16: 130 and 106, 42 and 32.
+// 16 (sample, head) x 257 tokens, hd 96, fp32: 67 and 52 us, 32 and 24; 2 x 2048, hd 128, bf16: 129 and 106, 46 and 35.
 struct Plan {
   bool many_q, many_k;
   int q_splits = 1, q_tiles, k_splits = 1, k_tiles;
