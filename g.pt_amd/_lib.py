@@ -176,8 +176,10 @@ _PROTOS = {
     "gpt_add_rmsnorm_bwd": ([C.POINTER(AddRmsNormBwd), vp], i32),
     "gpt_add_rmsnorm_bwd_workspace": ([i64, i64, C.POINTER(i64)], i32),
     "gpt_diff_attention": ([C.POINTER(DiffAttention), vp], i32),
+    "gpt_diff_attention_keep": ([C.POINTER(DiffAttention), vp, vp], i32),
     "gpt_diff_attention_workspace": ([i32] * 6 + [C.POINTER(i64)], i32),
     "gpt_diff_attention_bwd": ([C.POINTER(DiffAttention), C.POINTER(DiffAttentionBwd), vp], i32),
+    "gpt_diff_attention_bwd_kept": ([C.POINTER(DiffAttention), vp, C.POINTER(DiffAttentionBwd), vp], i32),
     "gpt_diff_attention_bwd_workspace": ([i32] * 6 + [C.POINTER(i64)], i32),
 }
 

@@ -16,6 +16,7 @@ struct Args {
   int64_t ldo, bso;
   float* lse;                 // [2][B][H][Tq], base 2, of the scaled scores
   void* out2;                 // [B][Tq][H * 2 hd]
+  bf16_t* rest;               // bf16, or NULL: [2][B][Tq][H * 2 hd], what the roundings of out and of out2 leave
   float* part;                // split forward: [splits][B * H][Tq][4 hd + 4]
   int B, Tq, Tk, H, splits, split_keys;
   float scale, c2;            // c2 = scale * log2(e): exp(scale s - m) = exp2(c2 s - m')
@@ -142,6 +143,15 @@ __device__ __forceinline__ void store4(bf16_t* p, const f32x4& v) {
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 __device__ __forceinline__ void store4(float* p, const f32x4& v) { *reinterpret_cast<f32x4*>(p) = v; }
+// the same, and what the rounding leaves to `rest` (NULL: nowhere)
+__device__ __forceinline__ void store4(bf16_t* p, bf16_t* rest, const f32x4& v) {
+  const uint32_t a = pack_bf16x2(v[0], v[1]), b = pack_bf16x2(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(a, b);
+  if (rest)
+    store4(rest, f32x4{v[0] - __uint_as_float(a << 16), v[1] - __uint_as_float(a & 0xffff0000u), v[2] - __uint_as_float(b << 16),
+                       v[3] - __uint_as_float(b & 0xffff0000u)});
+}
+__device__ __forceinline__ void store4(float* p, bf16_t*, const f32x4& v) { store4(p, v); }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }   // v_exp_f32, 1 ulp; exp2(-inf) = 0
 

@@ -30,6 +30,37 @@ constexpr int MAX_SPLITS = 512;
 template <typename T, int NW>
 constexpr int KEYS = sizeof(T) == 2 && NW > 1 ? 64 : 32;
 
+// column c of a row of Args::rest's plane (plane = the map whose output's rounding it is)
+template <int HD>
+__device__ __forceinline__ bf16_t* rest_row(const Args& a, int plane, int b, int qi, int c) {
+  return a.rest ? a.rest + (((int64_t)plane * a.B + b) * a.Tq + qi) * (a.H * 2 * HD) + c : nullptr;
+}
+
+// 16 columns of a row from the two lanes that hold them (this one columns 4 hh .. of the first 8 in x, of the next 8 in y), and what the
+// rounding leaves to `rest`.  bf16: the lanes exchange a half each, so that both store 16 bytes (16 samples of up to 515
+// tokens, hd 64, forward with all that it keeps: 62 us by 8 bytes, 52 by 16)
+template <bool KEPT>
+__device__ __forceinline__ void store_columns(bf16_t* p, bf16_t* rest, const f32x4& x, const f32x4& y, int hh) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float u = i < 2 ? x[2 * i] : y[2 * i - 4], v = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+    hi[i] = pack_bf16x2(u, v);
+    lo[i] = pack_bf16x2(u - __uint_as_float(hi[i] << 16), v - __uint_as_float(hi[i] & 0xffff0000u));
+  }
+  auto store = [&](bf16_t* dst, const uint32_t (&w)[4]) {
+    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    *reinterpret_cast<u32x4*>(dst + 8 * hh) = u32x4{a[0], b[0], a[1], b[1]};
+  };
+  store(p, hi);
+  if constexpr (KEPT) store(rest, lo);
+}
+template <bool>
+__device__ __forceinline__ void store_columns(float* p, bf16_t*, const f32x4& x, const f32x4& y, int hh) {
+  store4(p + 4 * hh, x);
+  store4(p + 8 + 4 * hh, y);
+}
+
 template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   using L = Tile<T, HD>;
@@ -203,34 +234,39 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   }
   // the second map's wave hands its normalised half over: [t][g] planes of 64 x 16 bytes, the same lane reads what a lane wrote
   const float inv = sum == 0.f ? 0.f : 1.f / sum;                            // no key: 0; NaN stays
-#pragma unroll
-  for (int t = 0; t < CT; ++t) o[t] *= inv;
   f32x4* ex = reinterpret_cast<f32x4*>(smem) + grp * (CT * 4 * 64) + lane;
   tile_barrier<0>();
   if (m == 1) {
 #pragma unroll
     for (int t = 0; t < CT; ++t)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) ex[(t * 4 + g) * 64] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+      for (int g = 0; g < 4; ++g) ex[(t * 4 + g) * 64] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]} * inv;
   }
   tile_barrier<0>();
   if (!qok) return;
   if (a.lse && hh == 0) a.lse[((int64_t)m * a.B * a.H + pair) * a.Tq + qi] = sum == 0.f ? INFINITY : top * a.c2 + __builtin_amdgcn_logf(sum);
-  if (m == 0) {
-    const float lam = a.lam[h];
-    T* orow = (T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD + 4 * hh;
+  auto finish = [&](auto kept) {                                               // the rows of map m, with what their rounding leaves or without
+    const bool second = m == 1;
+    const float lam = second ? 0.f : a.lam[h];
+    T* orow = second ? (T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD
+                     : (T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD;
+    bf16_t* rrow = kept.value ? rest_row<HD>(a, m, b, qi, h * 2 * HD) : nullptr;
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+    for (int i = 0; i < 2 * CT; ++i) {
+      f32x4 x[2];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        store4(orow + t * 32 + 8 * g, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]} - ex[(t * 4 + g) * 64] * lam);
-  } else if (a.out2) {
-    T* orow = (T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD + 4 * hh;
-#pragma unroll
-    for (int t = 0; t < CT; ++t)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) store4(orow + t * 32 + 8 * g, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]});
-  }
+      for (int k = 0; k < 2; ++k) {
+        const int t = i / 2, g = 2 * (i & 1) + k;
+        x[k] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]} * inv;
+        if (!second) x[k] -= ex[(t * 4 + g) * 64] * lam;
+      }
+      store_columns<kept.value>(orow + i * 16, rrow + i * 16, x[0], x[1], hh);
+      PIN();                                                                   // (all of `ex` read at once would spill)
+    }
+  };
+  if (m == 1 && !a.out2) return;
+  if (sizeof(T) == 2 && a.rest) finish(std::integral_constant<bool, sizeof(T) == 2>{});
+  else finish(std::integral_constant<bool, false>{});
 }
 
 // joins few splits: one wave per (sample, head, query); lane owns 4 columns of 2 hd
@@ -265,8 +301,9 @@ __global__ __launch_bounds__(256) void join_few_kernel(Args a) {
       }
     }
     const f32x4 first = sum[0] == 0.f ? o[0] : o[0] / sum[0], second = sum[1] == 0.f ? o[1] : o[1] / sum[1];
-    store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD + lane * 4, first - second * a.lam[h]);
-    if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD + lane * 4, second);
+    const int c = h * 2 * HD + lane * 4;
+    store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + c, rest_row<HD>(a, 0, b, qi, c), first - second * a.lam[h]);
+    if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + c, rest_row<HD>(a, 1, b, qi, c), second);
   }
   if (a.lse && lane < 2) {
     const float s = lane ? sum[1] : sum[0], t = lane ? top[1] : top[0];
@@ -326,8 +363,9 @@ __global__ __launch_bounds__(256) void join_many_kernel(Args a) {
       first += share[q * COLS + tid];
       second += share[q * COLS + tid + HD / 2];
     }
-    store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + h * 2 * HD + tid * 4, first - second * a.lam[h]);
-    if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + h * 2 * HD + tid * 4, second);
+    const int col = h * 2 * HD + tid * 4;
+    store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + col, rest_row<HD>(a, 0, b, qi, col), first - second * a.lam[h]);
+    if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + col, rest_row<HD>(a, 1, b, qi, col), second);
   }
   if (a.lse && tid < 2) {
     const float s = total[tid][1];
@@ -416,6 +454,13 @@ int make_args(const gpt_diff_attention_t* p, const char* who, Args* a) {
   return 0;
 }
 
+int check_rest(const gpt_diff_attention_t* p, void* rest, const char* who, Args* a) {
+  GPT_REQUIRE(!rest || (p->dtype == GPT_BF16 && p->out2), "%s: rest belongs to a bf16 call that keeps out2", who);
+  GPT_REQUIRE((uintptr_t)rest % 16 == 0, "%s: misaligned operand", who);
+  a->rest = (bf16_t*)rest;
+  return 0;
+}
+
 }  // namespace diffattn
 
 using namespace diffattn;
@@ -433,10 +478,13 @@ extern "C" int gpt_diff_attention_workspace(int dtype, int B, int Tq, int Tk, in
   return 0;
 }
 
-extern "C" int gpt_diff_attention(const gpt_diff_attention_t* p, void* stream) {
+extern "C" int gpt_diff_attention(const gpt_diff_attention_t* p, void* stream) { return gpt_diff_attention_keep(p, nullptr, stream); }
+
+extern "C" int gpt_diff_attention_keep(const gpt_diff_attention_t* p, void* rest, void* stream) {
   const char* who = "gpt_diff_attention";
   Args a;
   if (int st = make_args(p, who, &a)) return st;
+  if (int st = check_rest(p, rest, who, &a)) return st;
   if (p->Tq <= SHORT && p->Tk <= SHORT) return short_attention(a, p->dtype, p->hd, false, (hipStream_t)stream);
   const int64_t need = fwd_workspace(p->dtype, p->B, p->Tq, p->Tk, p->n_head, p->hd);
   if (need > 0) {

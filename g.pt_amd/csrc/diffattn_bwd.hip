@@ -17,6 +17,7 @@
 
 namespace diffattn {
 int make_args(const gpt_diff_attention_t* p, const char* who, Args* a);
+int check_rest(const gpt_diff_attention_t* p, void* rest, const char* who, Args* a);
 
 namespace {
 
@@ -144,7 +145,9 @@ __device__ __forceinline__ Frag<T> col16(const char* tile, int cb, int t) {
   return f;
 }
 
-// per (sample, head, query) the two log-sum-exps and D_1 = dO . (out + lam out2), D_2 = dO . out2: 16 lanes each
+// per (sample, head, query) the two log-sum-exps and D_1 = dO . (out + lam out2), D_2 = dO . out2: 16 lanes each.  In bf16 with what
+// their roundings left added back: dS = P (dP - D) is small where a row has few keys or one that outweighs the others, and D from the rounded
+// outputs is off by 2^-9 of dP there (a row of one key has dS = 0; 16 samples of up to 515 tokens: dQ 1.71e-3 rms off, 1.66e-3 with it)
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void stats_kernel(Args a, f32x4* stats) {
   constexpr int CH = 2 * HD * sizeof(T) / 16, PER = 16 / sizeof(T);
@@ -161,14 +164,20 @@ __global__ __launch_bounds__(256) void stats_kernel(Args a, f32x4* stats) {
     const int ch = c * 16 + lane;
     if (ch >= CH) break;
     const u32x4 x = reinterpret_cast<const u32x4*>(g)[ch], y = reinterpret_cast<const u32x4*>(o)[ch], z = reinterpret_cast<const u32x4*>(o2)[ch];
+    u32x4 ry = {0u, 0u, 0u, 0u}, rz = ry;
+    if (sizeof(T) == 2 && a.rest) {
+      const bf16_t* r = a.rest + row * (2 * HD);
+      ry = reinterpret_cast<const u32x4*>(r)[ch];
+      rz = reinterpret_cast<const u32x4*>(r + rows * (2 * HD))[ch];
+    }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       float xv, yv, zv;
       if constexpr (sizeof(T) == 2) {
         const int sh = (j & 1) ? 0 : 16;
         xv = __uint_as_float((x[j >> 1] << sh) & 0xffff0000u);
-        yv = __uint_as_float((y[j >> 1] << sh) & 0xffff0000u);
-        zv = __uint_as_float((z[j >> 1] << sh) & 0xffff0000u);
+        yv = __uint_as_float((y[j >> 1] << sh) & 0xffff0000u) + __uint_as_float((ry[j >> 1] << sh) & 0xffff0000u);
+        zv = __uint_as_float((z[j >> 1] << sh) & 0xffff0000u) + __uint_as_float((rz[j >> 1] << sh) & 0xffff0000u);
       } else {
         xv = __uint_as_float(x[j]); yv = __uint_as_float(y[j]); zv = __uint_as_float(z[j]);
       }
@@ -618,9 +627,14 @@ extern "C" int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk
 }
 
 extern "C" int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_diff_attention_bwd_t* p, void* stream) {
+  return gpt_diff_attention_bwd_kept(f, nullptr, p, stream);
+}
+
+extern "C" int gpt_diff_attention_bwd_kept(const gpt_diff_attention_t* f, const void* rest, const gpt_diff_attention_bwd_t* p, void* stream) {
   const char* who = "gpt_diff_attention_bwd";
   Args a;
   if (int st = make_args(f, who, &a)) return st;
+  if (int st = check_rest(f, const_cast<void*>(rest), who, &a)) return st;
   GPT_REQUIRE(p && p->dout && p->dq && p->dk && p->dv && p->dlam, "%s: null operand", who);
   const bool is_short = f->Tq <= SHORT && f->Tk <= SHORT;
   GPT_REQUIRE(is_short || (f->lse && f->out2), "%s: needs the forward's lse and out2", who);

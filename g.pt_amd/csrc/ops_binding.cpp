@@ -42,9 +42,9 @@ struct Entries {
   decltype(&gpt_add_rmsnorm) add_rmsnorm = nullptr;
   decltype(&gpt_add_rmsnorm_bwd) add_rmsnorm_bwd = nullptr;
   decltype(&gpt_add_rmsnorm_bwd_workspace) add_rmsnorm_bwd_workspace = nullptr;
-  decltype(&gpt_diff_attention) diff_attention = nullptr;
+  decltype(&gpt_diff_attention_keep) diff_attention = nullptr;
   decltype(&gpt_diff_attention_workspace) diff_attention_workspace = nullptr;
-  decltype(&gpt_diff_attention_bwd) diff_attention_bwd = nullptr;
+  decltype(&gpt_diff_attention_bwd_kept) diff_attention_bwd = nullptr;
   decltype(&gpt_diff_attention_bwd_workspace) diff_attention_bwd_workspace = nullptr;
 } lib;
 
@@ -58,9 +58,9 @@ void bind_library(uintptr_t handle) {
   get(lib.add_rmsnorm, "gpt_add_rmsnorm");
   get(lib.add_rmsnorm_bwd, "gpt_add_rmsnorm_bwd");
   get(lib.add_rmsnorm_bwd_workspace, "gpt_add_rmsnorm_bwd_workspace");
-  get(lib.diff_attention, "gpt_diff_attention");
+  get(lib.diff_attention, "gpt_diff_attention_keep");
   get(lib.diff_attention_workspace, "gpt_diff_attention_workspace");
-  get(lib.diff_attention_bwd, "gpt_diff_attention_bwd");
+  get(lib.diff_attention_bwd, "gpt_diff_attention_bwd_kept");
   get(lib.diff_attention_bwd_workspace, "gpt_diff_attention_bwd_workspace");
 }
 
@@ -448,7 +448,7 @@ struct AttentionCall {
 };
 
 struct AttentionOut {
-  Tensor out, lse, out2;
+  Tensor out, lse, out2, rest;
 };
 
 AttentionOut attention_forward(const Attention& a, bool keep) {
@@ -468,6 +468,7 @@ AttentionOut attention_forward(const Attention& a, bool keep) {
     o.lse = at::empty({2, a.B(), a.n_head, a.Tq()}, opt.dtype(at::kFloat));
     o.out2 = at::empty(o.out.sizes(), opt);
     c.lse = o.lse.data_ptr<float>(); c.out2 = o.out2.data_ptr();
+    if (c.dtype == GPT_BF16) o.rest = at::empty({2, a.B(), a.Tq(), a.q.size(2)}, opt);
   }
   int64_t bytes = 0;
   check(lib.diff_attention_workspace(c.dtype, c.B, c.Tq, c.Tk, c.n_head, c.hd, &bytes), "gpt_diff_attention_workspace");
@@ -476,14 +477,14 @@ AttentionOut attention_forward(const Attention& a, bool keep) {
     ws = at::empty({bytes}, opt.dtype(at::kByte));
     c.ws = ws.data_ptr(); c.ws_bytes = bytes;
   }
-  check(lib.diff_attention(&c, stream_of(a.q)), "gpt_diff_attention");
+  check(lib.diff_attention(&c, o.rest.defined() ? o.rest.data_ptr() : nullptr, stream_of(a.q)), "gpt_diff_attention");
   return o;
 }
 
 struct DiffAttentionBackward : OnceNode {
   std::string name() const override { return "GptDiffAttentionBackward"; }
-  bool fused, has_lengths, kept;
-  SavedVariable q, k, v, lam, lengths, out, lse, out2;                 // fused: q holds the whole projection
+  bool fused, has_lengths, kept, has_rest;
+  SavedVariable q, k, v, lam, lengths, out, lse, out2, rest;           // fused: q holds the whole projection
   int n_head;
   float scale;
   variable_list apply(variable_list&& grads) override {
@@ -521,7 +522,7 @@ struct DiffAttentionBackward : OnceNode {
     AttentionCall call(a);
     const Tensor o = kept ? out.unpack(shared_from_this()) : dq;         // not read where nothing was kept
     call.c.out = o.data_ptr(); call.c.ldo = o.stride(1); call.c.bso = o.stride(0);
-    const Tensor lse_v = kept ? lse.unpack() : Tensor(), out2_v = kept ? out2.unpack() : Tensor();
+    const Tensor lse_v = kept ? lse.unpack() : Tensor(), out2_v = kept ? out2.unpack() : Tensor(), rest_v = has_rest ? rest.unpack() : Tensor();
     if (kept) { call.c.lse = lse_v.data_ptr<float>(); call.c.out2 = out2_v.data_ptr(); }
     const Tokens gt(g);
     gpt_diff_attention_bwd_t b{};
@@ -535,12 +536,12 @@ struct DiffAttentionBackward : OnceNode {
           "gpt_diff_attention_bwd_workspace");
     const Tensor ws = at::empty({bytes}, a.lam.options().dtype(at::kByte).requires_grad(false));
     b.ws = ws.data_ptr(); b.ws_bytes = bytes;
-    check(lib.diff_attention_bwd(&call.c, &b, stream_of(first)), "gpt_diff_attention_bwd");
+    check(lib.diff_attention_bwd(&call.c, has_rest ? rest_v.data_ptr() : nullptr, &b, stream_of(first)), "gpt_diff_attention_bwd");
     return res;
   }
   void release_variables() override {
     const auto lock = hold();
-    for (SavedVariable* s : {&q, &k, &v, &lam, &lengths, &out, &lse, &out2}) s->reset_data();
+    for (SavedVariable* s : {&q, &k, &v, &lam, &lengths, &out, &lse, &out2, &rest}) s->reset_data();
   }
 };
 
@@ -578,6 +579,7 @@ Tensor diff_attention_any(const char* who, const Tensor* qkv, const Tensor& q, c
     node->fused = qkv != nullptr;
     node->has_lengths = a.lengths.defined();
     node->kept = o.lse.defined();
+    node->has_rest = o.rest.defined();
     node->n_head = a.n_head;
     node->scale = a.scale;
     torch::autograd::create_gradient_edge(o.out, node);
@@ -586,6 +588,7 @@ Tensor diff_attention_any(const char* who, const Tensor* qkv, const Tensor& q, c
     node->lam = SavedVariable(a.lam, false);
     if (a.lengths.defined()) node->lengths = SavedVariable(a.lengths, false);
     if (node->kept) { node->out = SavedVariable(o.out, true); node->lse = SavedVariable(o.lse, false); node->out2 = SavedVariable(o.out2, false); }
+    if (node->has_rest) node->rest = SavedVariable(o.rest, false);
   }
   return o.out;
 }

@@ -608,6 +608,10 @@ typedef struct {
 } gpt_diff_attention_t;
 int gpt_diff_attention_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes);
 int gpt_diff_attention(const gpt_diff_attention_t* a, void* stream);
+/* The same with `rest` (GPT_BF16 with out2 kept, 16-byte aligned; else NULL): bf16 [2][B][Tq][n_head * 2 * hd], what the roundings of out and
+ * of out2 left.  With it the backward has the row sums D_i to 16 bits; without, from the rounded out and out2, to 8 (dq and dk of rows
+ * that hardly attend to more than one key are then off by 2^-9 of dP's size). */
+int gpt_diff_attention_keep(const gpt_diff_attention_t* a, void* rest, void* stream);
 
 /* Its backward, `f` being the forward's descriptor (out, lse, out2 as it left them).  With dO = dL/dout and dP = dO V^T,
  * D_i = rowsum(P_i dP), dS_1 = P_1 (dP - D_1), dS_2 = -lam P_2 (dP - D_2):
@@ -623,6 +627,7 @@ typedef struct {
 } gpt_diff_attention_bwd_t;
 int gpt_diff_attention_bwd_workspace(int dtype, int B, int Tq, int Tk, int n_head, int hd, int64_t* host_bytes);
 int gpt_diff_attention_bwd(const gpt_diff_attention_t* f, const gpt_diff_attention_bwd_t* g, void* stream);
+int gpt_diff_attention_bwd_kept(const gpt_diff_attention_t* f, const void* rest, const gpt_diff_attention_bwd_t* g, void* stream);
 
 /* ---- dropout in the denoiser's training step ------------------------------------------------------------------------------------
  * gpt_attention_rows with dropout on the softmax probabilities (Gpt/models/transformer.py:43-47), and its backward (dqkv is stored):
