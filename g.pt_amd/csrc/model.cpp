@@ -114,7 +114,10 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
     const char* e = getenv("GPT_PRUNE_LAST");   // 0: all rows through the last Block (cross-check, A/B)
     return !e || atoi(e) != 0;
   }();
-  const bool prune = prune_on && !keep && !drop && L > 0 && m->n_out_tok < T && (size_t)(T - m->n_out_tok) * 4 * es >= (size_t)m->n_out_tok * 4;
+  // With dropout this forward prunes exactly where the training forward does: the last Block's residual masks are indexed by the rows
+  // that it works on, and one seed means one set of masks whether or not gradients are recorded
+  const bool prune = !keep && (drop ? prune_last_train(m, B)
+                                    : prune_on && L > 0 && m->n_out_tok < T && (size_t)(T - m->n_out_tok) * 4 * es >= (size_t)m->n_out_tok * 4);
 
   // ln_in + position embedding (transformer.py:226, 308-309), then the first Block's ln1: one launch in the inference forward
   // (no statistics kept), two otherwise
@@ -181,14 +184,14 @@ static int denoiser_forward(const gpt_model_t* m, const gpt_workspace_t* ws, con
       // Block's FLOPs.  Same arithmetic per row; what changes is which kernel instance a GEMM of that height takes.
       // (r01 measured +-0 for this at B = 320 on the kernels of the time; with gemm128.hip and the K-span passes: section 4.)
       const int To = m->n_out_tok, Mc = B * To;
-      float* xc = reinterpret_cast<float*>((char*)ws->act + (size_t)Mc * 4 * d * es);   // the part of `act` the compact rows leave free
-      CHECK(gpt_attention_rows(dt, qkv, att, B, T, To, m->n_head, d / m->n_head, stream));
+      // xc: the part of `act` that the compact rows leave free, where that is enough; with dropout the encoder's output, which no later
+      // step takes up again there
+      float* xc = drop ? ws->enc : reinterpret_cast<float*>((char*)ws->act + (size_t)Mc * 4 * d * es);
+      CHECK(attention(To));
       CHECK(gpt_gather_token_rows(xin, xc, B, T, To, d, stream));
-      CHECK(gpt_gemm_resadd_layernorm(dt, att, d, ly.wproj, d, ly.bproj, xc, d, xc, d, ly.ln2_w, ly.ln2_b, h2, nullptr, nullptr, Mc, d, d,
-                                      1e-5f, stream));
+      CHECK(residual(SITE_PROJ, att, d, ly.wproj, ly.bproj, xc, xc, ly.ln2_w, ly.ln2_b, h2, nullptr, nullptr, Mc));
       CHECK(gpt_gemm_nt(dt, h2, d, ly.w1, d, ly.b1, act, 4 * d, nullptr, 0, Mc, 4 * d, d, GPT_EPI_GELU, stream));
-      CHECK(gpt_gemm_resadd_layernorm(dt, act, 4 * d, ly.w2, 4 * d, ly.b2, xc, d, xc, d, m->ln_f_w, m->ln_f_b, ws->hf, nullptr, nullptr, Mc, d,
-                                      4 * d, 1e-5f, stream));
+      CHECK(residual(SITE_MLP, act, 4 * d, ly.w2, ly.b2, xc, xc, m->ln_f_w, m->ln_f_b, ws->hf, nullptr, nullptr, Mc));
       CHECK(wait_ready(m->dec_ready, stream));
       return gpt_decode_tokens(dt, To, ws->hf, To, m->dec_w, m->dec_n, m->dec_off, x_prev, out, B, d, m->D, stream);
     }

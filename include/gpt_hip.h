@@ -640,7 +640,8 @@ int gpt_attention_dropout_bwd(int dtype, const void* qkv, const void* dy, void* 
 /* The probabilities of transformer.py:34-72, 302-314 (embd: position-embedded tokens; attn: attention probabilities; resid: the
  * outputs of both residual branches of a Block).  The masks of a step take the offsets offset .. offset + 3 n_layer: site 0 = embd,
  * 1 + 3 l, 2 + 3 l, 3 + 3 l = Block l's attention, projection and MLP; forward and backward of a step are given the same struct.
- * (Where the last Block works on the decoded tokens' rows alone, its two residual masks are those of the compact rows.) */
+ * (GPT_BF16 with d % 256 == 0: the last Block works on the decoded tokens' rows alone and its two residual masks are those of the compact
+ * rows, in the training forward as in the one without kept activations.) */
 typedef struct {
   double embd, attn, resid;
   uint64_t seed, offset;

@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 import torch.nn.functional as F
+import torch.utils.checkpoint
 
 import gpt_amd
 from gpt_amd import _lib as L
@@ -242,3 +243,31 @@ def test_train_step_uses_the_masks(dtype, n_embd, n_head):
         assert float((got[0][k].reshape(w.shape) - w).abs().max()) <= 2e-5 * float(w.abs().max()) + 1e-12, k
     k = "decoder.blocks.1.mlp.0.weight"
     assert float(F.cosine_similarity(got[0][k].flatten(), got[1][k].flatten(), 0)) < 0.999
+
+
+@gpu
+@pytest.mark.parametrize("pd", [PDROP, dict(embd_pdrop=0.0, attn_pdrop=0.0, resid_pdrop=0.5)], ids=["all", "resid"])
+@pytest.mark.parametrize("B", [1, 5])
+def test_one_seed_means_one_set_of_masks_with_and_without_gradients(B, pd):
+    """256 columns in bf16: the training forward takes the last Block on the decoded tokens' rows, and so does the forward without gradients
+    (activation checkpointing runs both).  The bar is that of 192 columns, where no rows are left out: the two forwards' kernels
+    round differently, a mask of other rows changes the output by its own size."""
+    m, plan, _ = model("bf16", 256, 4, pd)
+    inputs = make_inputs("mnist_small", B=B, seed=19)
+    c = normal(8, *inputs[0].shape, device="cpu")
+    _, a, grads = steps(m, inputs, c, seed=1)
+    args = [v.to(DEV) for v in inputs]
+    call = lambda x: m(x, args[1], args[2], loss_prev=args[3], x_prev=args[4])                              # noqa: E731
+    torch.manual_seed(1)
+    with torch.no_grad():
+        free = call(args[0]).cpu()
+    assert rel_err(free - inputs[4], a - inputs[4]) < 2e-2
+    # checkpointed: a pass without gradients, then one with them under the same generator state
+    torch.manual_seed(1)
+    for p in m.parameters():
+        p.grad = None
+    out = torch.utils.checkpoint.checkpoint(call, args[0].clone().requires_grad_(), use_reentrant=True)
+    assert rel_err(out.detach().cpu() - inputs[4], a - inputs[4]) < 2e-2
+    (out * c.to(DEV)).sum().backward()
+    for k, p in m.named_parameters():
+        assert torch.equal(p.grad.float().cpu(), grads[k]) or rel_err(p.grad.float().cpu(), grads[k]) < 1e-4, k
