@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
@@ -77,7 +78,15 @@ int code(const Tensor& t, const char* who, const char* name) {
   fail(who, name, " must be float32 or bfloat16 (got ", t.scalar_type(), ")");
 }
 
+// What the nodes below do not carry on is refused, not dropped: the tangents of forward-mode differentiation
+void plain_call(const char* who, std::initializer_list<const Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors)
+    OPS_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), who, "forward-mode differentiation is not implemented");
+}
+
 void same_device(const char* who, std::initializer_list<const Tensor*> tensors) {
+  plain_call(who, tensors);
   const Tensor* first = nullptr;
   for (const Tensor* t : tensors) {
     if (!t || !t->defined()) continue;
@@ -143,6 +152,7 @@ struct OnceNode : torch::autograd::Node {
   // (the node's members are read under its lock: a graph may be run by one thread and released by another)
   std::lock_guard<std::mutex> hold() { return std::lock_guard<std::mutex>(mutex_); }
   void once(const char* who, const variable_list& grads) {
+    for (const Tensor& g : grads) plain_call(who, {&g});
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor& g : grads)
       if (g.defined() && g.requires_grad())
@@ -600,6 +610,7 @@ Tensor diff_attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
 
 Tensor diff_attention_qkv(const Tensor& qkv, const Tensor& lam, int64_t n_head, const OptTensor& lengths, const std::optional<double>& scale) {
   const char* who = "diff_attention_qkv";
+  plain_call(who, {&qkv});                                                // (the detached ranges below have no tangent)
   OPS_CHECK(qkv.dim() == 3 && qkv.size(2) % 3 == 0, who, "qkv must be a [B, T, 3 w] tensor (got ", qkv.sizes(), ")");
   const int64_t w = qkv.size(2) / 3;
   const Tensor flat = qkv.detach();

@@ -888,3 +888,41 @@ def test_refusals_of_the_python_entries():
         x = h.clone().requires_grad_()
         g, = torch.autograd.grad(ops.rms_norm(x, w).pow(2).sum(), x, create_graph=True)
         g.sum().backward()
+
+
+def floating_calls(x):
+    """Every entry, with `x` [4, 192] in the place of each floating argument in turn."""
+    w, lam, q = torch.ones(192, device=x.device), torch.zeros(1, device=x.device), torch.zeros(4, 192, device=x.device)
+    a, b = x[None].narrow(2, 0, 64), q[None].narrow(2, 0, 64)
+    return [lambda: ops.dropout(x, 0.1, 0), lambda: ops.dropout_add(x, q, 0.1, 0), lambda: ops.dropout_add(q, x, 0.1, 0), lambda: ops.rms_norm(x, w),
+            lambda: ops.rms_norm(q, x[0]), lambda: ops.add_rms_norm(x, q, w), lambda: ops.add_rms_norm(q, x, w), lambda: ops.add_rms_norm(q, q, x[0]),
+            lambda: ops.add_rms_norm_mx8(x, q, w), lambda: ops.add_rms_norm_mx8(q, x, w), lambda: ops.rms_norm_mx8(x, w),
+            lambda: ops.diff_attention(a, b, b, lam, 1), lambda: ops.diff_attention(b, a, b, lam, 1), lambda: ops.diff_attention(b, b, a, lam, 1),
+            lambda: ops.diff_attention(b, b, b, x[0, :1], 1), lambda: ops.diff_attention_qkv(x[None], lam, 1), lambda: ops.diff_attention_qkv(q[None], x[0, :1], 1)]
+
+
+def check_forward_mode_is_refused(device):
+    import torch.autograd.forward_ad as fwd
+    x = torch.zeros(4, 192, device=device)
+    with fwd.dual_level():
+        for call in floating_calls(fwd.make_dual(x, torch.ones_like(x))):
+            with pytest.raises(L.GptHipError, match="forward-mode"):
+                call()
+
+
+def test_forward_mode_is_refused():
+    """A tangent is an error, not silently dropped (before the check of the device: no GPU is needed)."""
+    check_forward_mode_is_refused("cpu")
+
+
+@gpu
+def test_forward_mode_is_refused_on_the_gpu():
+    import torch.autograd.forward_ad as fwd
+    check_forward_mode_is_refused(DEV)
+    with fwd.dual_level():                               # a level without a tangent on any argument is an ordinary call
+        assert all(call() is not None for call in floating_calls(normal(1, 4, 192)))
+        # nor does a backward pass drop the tangent of its gradient
+        x, w, lam = normal(1, 2, 4, 192).requires_grad_(), torch.ones(192, device=DEV), torch.zeros(1, device=DEV)
+        for out in (ops.dropout(x, 0.1, 0), ops.rms_norm(x, w), ops.diff_attention_qkv(x, lam, 1)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, x, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
