@@ -6,8 +6,11 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 
@@ -78,8 +81,25 @@ int code(const Tensor& t, const char* who, const char* name) {
   fail(who, name, " must be float32 or bfloat16 (got ", t.scalar_type(), ")");
 }
 
+// A tracer would record the allocation of the result and none of the launches that fill it: a graph of uninitialised memory.  Refused are
+// torch.jit.trace, the modes of torch that trace (fake tensors, make_fx with and without pre_dispatch, functionalization) and the
+// transforms' wrapped tensors.  A caller's own dispatch mode (a FLOP counter, selective checkpointing) sees the allocation alone as well, but
+// the call's result is right under it.
+void not_traced(const char* who, std::initializer_list<const Tensor*> tensors) {
+  using c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::BatchedNestedTensor, c10::DispatchKey::Functionalize,
+                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchDynamicLayerFrontMode});
+  bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  if (TorchDispatchModeTLS::any_modes_set())
+    for (Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL}) traced |= TorchDispatchModeTLS::get_mode(k).has_value();
+  for (const Tensor* t : tensors) traced |= t && t->defined() && t->key_set().has_any(wrapped);
+  OPS_CHECK(!traced, who, "tracing and function transforms (jit.trace, make_fx, fake tensors, torch.func) are not implemented");
+}
+
 // What the nodes below do not carry on is refused, not dropped: the tangents of forward-mode differentiation
 void plain_call(const char* who, std::initializer_list<const Tensor*> tensors) {
+  not_traced(who, tensors);
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : tensors)
     OPS_CHECK(!t || !t->defined() || !t->_fw_grad(/*level=*/0).defined(), who, "forward-mode differentiation is not implemented");

@@ -926,3 +926,35 @@ def test_forward_mode_is_refused_on_the_gpu():
         for out in (ops.dropout(x, 0.1, 0), ops.rms_norm(x, w), ops.diff_attention_qkv(x, lam, 1)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, x, fwd.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def check_tracing_is_refused(device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.zeros(4, 192, device=device)
+    for i in range(len(floating_calls(x))):
+        call = lambda v: floating_calls(v)[i]()                                                               # noqa: E731,B023
+        for trace in (lambda: torch.jit.trace(call, (x,), check_trace=False), lambda: make_fx(call)(x), lambda: make_fx(call, pre_dispatch=True)(x),
+                      lambda: make_fx(call, tracing_mode="fake")(x), lambda: torch.func.functionalize(call)(x)):
+            with pytest.raises(L.GptHipError, match="tracing"):
+                trace()
+    for transform in (torch.vmap, torch.func.grad):
+        with pytest.raises(L.GptHipError, match="tracing"):
+            transform(lambda v: ops.dropout(v, 0.1, 0).sum())(x)
+
+
+def test_tracing_is_refused():
+    """A trace would hold an allocation and no launch (before the check of the device: no GPU is needed)."""
+    check_tracing_is_refused("cpu")
+
+
+@gpu
+def test_tracing_is_refused_on_the_gpu_and_a_flop_counter_is_not():
+    from torch.utils.flop_counter import FlopCounterMode
+    check_tracing_is_refused(DEV)
+    x = normal(1, 4, 192)
+    want = [call() for call in floating_calls(x)]
+    with FlopCounterMode(display=False):
+        got = [call() for call in floating_calls(x)]
+    for a, b in zip(want, got):
+        for u, v in zip(a, b) if isinstance(a, tuple) else ((a, b),):
+            assert torch.equal(u.view(torch.uint8), v.view(torch.uint8))
