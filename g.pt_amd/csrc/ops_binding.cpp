@@ -167,17 +167,21 @@ Drop make_drop(const char* who, double p, uint64_t seed, uint64_t offset, const 
   return d;
 }
 
-// a node whose backward is not itself differentiable
+bool wants_grad(const Tensor* t) { return t && t->defined() && t->requires_grad(); }
+
+// a node whose backward is not itself differentiable: with create_graph, gradients that would have a graph - because the incoming one has,
+// or because they depend on inputs that require one themselves (`curved`) - are an error, not constants
 struct OnceNode : torch::autograd::Node {
   // (the node's members are read under its lock: a graph may be run by one thread and released by another)
   std::lock_guard<std::mutex> hold() { return std::lock_guard<std::mutex>(mutex_); }
   void once(const char* who, const variable_list& grads) {
     for (const Tensor& g : grads) plain_call(who, {&g});
     if (!at::GradMode::is_enabled()) return;
-    for (const Tensor& g : grads)
-      if (g.defined() && g.requires_grad())
-        throw std::runtime_error(c10::str(who, ": the gradient cannot be differentiated again (create_graph)"));
+    bool graph = curved;
+    for (const Tensor& g : grads) graph |= g.defined() && g.requires_grad();
+    if (graph) throw std::runtime_error(c10::str(who, ": the gradient cannot be differentiated again (create_graph)"));
   }
+  bool curved = false;
 };
 
 template <typename N>
@@ -391,6 +395,7 @@ NormOut norm_autograd(const char* who, const Tensor* h, const Tensor& resid, con
   NormOut o = norm_forward(who, h, resid, weight, eps, drop, y_type, grad);
   if (grad) {
     auto node = make_node<AddRmsNormBackward>({h, &resid, &weight});
+    node->curved = wants_grad(h) || wants_grad(&resid);                  // (the weight alone: its gradient does not depend on it)
     node->y_type = y_type;
     node->has_h = h != nullptr;
     node->has_counter = counter != nullptr;
@@ -606,6 +611,8 @@ Tensor diff_attention_any(const char* who, const Tensor* qkv, const Tensor& q, c
   AttentionOut o = attention_forward(a, grad);
   if (grad) {
     auto node = qkv ? make_node<DiffAttentionBackward>({qkv, &a.lam}) : make_node<DiffAttentionBackward>({&q, &k, &v, &a.lam});
+    // (v alone, or lam alone: linear in it)
+    node->curved = wants_grad(qkv) || wants_grad(&q) || wants_grad(&k) || (wants_grad(&v) && wants_grad(&a.lam));
     node->fused = qkv != nullptr;
     node->has_lengths = a.lengths.defined();
     node->kept = o.lse.defined();

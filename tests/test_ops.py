@@ -958,3 +958,30 @@ def test_tracing_is_refused_on_the_gpu_and_a_flop_counter_is_not():
     for a, b in zip(want, got):
         for u, v in zip(a, b) if isinstance(a, tuple) else ((a, b),):
             assert torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("T", [5, 40])
+def test_gradients_with_a_graph_are_refused_and_never_constants(T):
+    """create_graph with a constant incoming gradient: what depends on its own inputs raises; what is linear in the inputs that require a
+    gradient has none to keep and is the ordinary gradient."""
+    leaf = lambda s, *n: normal(s, *n).requires_grad_()                                                      # noqa: E731
+    x, h, w, lam = leaf(1, 1, T, 192), leaf(2, 1, T, 192), leaf(3, 192), torch.rand(1, device=DEV).requires_grad_()
+    q, k, v = (leaf(s, 1, T, 64) for s in (4, 5, 6))
+    c = lambda t: t.detach()                                                                                 # noqa: E731
+    att = ops.diff_attention
+    curved = [(ops.rms_norm(x, w), (x, w)), (ops.rms_norm(x, c(w)), (x,)), (ops.rms_norm(x, w), (w,)), (ops.add_rms_norm(h, c(x), c(w))[0], (h,)),
+              (ops.add_rms_norm(c(h), x, w)[1], (x,)), (att(q, c(k), c(v), c(lam), 1), (q,)), (att(c(q), k, c(v), c(lam), 1), (k,)),
+              (att(c(q), c(k), v, lam, 1), (v, lam)), (att(q, k, v, lam, 1), (v,)), (ops.diff_attention_qkv(x, c(lam), 1), (x,))]
+    for out, leaves in curved:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out, leaves, torch.ones_like(out), create_graph=True, retain_graph=True)
+        assert all(g is not None for g in torch.autograd.grad(out, leaves, torch.ones_like(out)))             # without a graph: as before
+    linear = [(ops.dropout_add(h, x, 0.3, 1), (h, x)), (ops.rms_norm(c(x), w), (w,)), (att(c(q), c(k), v, c(lam), 1), (v,)),
+              (att(c(q), c(k), c(v), lam, 1), (lam,))]
+    for out, leaves in linear:
+        g = torch.ones_like(out)
+        kept = torch.autograd.grad(out, leaves, g, create_graph=True, retain_graph=True)
+        assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(kept, torch.autograd.grad(out, leaves, g, retain_graph=True)))
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out, leaves, g.requires_grad_(), create_graph=True)
