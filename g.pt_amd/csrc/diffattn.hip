@@ -233,7 +233,7 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
     return;
   }
   // the second map's wave hands its normalised half over: [t][g] planes of 64 x 16 bytes, the same lane reads what a lane wrote
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;                            // no key: 0; NaN stays
+  const float inv = n > 0 ? 1.f / sum : 0.f;                                 // no key: 0; nothing but scores of -inf: 0 / 0
   f32x4* ex = reinterpret_cast<f32x4*>(smem) + grp * (CT * 4 * 64) + lane;
   tile_barrier<0>();
   if (m == 1) {
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(NW * 128) void fwd_kernel(Args a) {
   }
   tile_barrier<0>();
   if (!qok) return;
-  if (a.lse && hh == 0) a.lse[((int64_t)m * a.B * a.H + pair) * a.Tq + qi] = sum == 0.f ? INFINITY : top * a.c2 + __builtin_amdgcn_logf(sum);
+  if (a.lse && hh == 0) a.lse[((int64_t)m * a.B * a.H + pair) * a.Tq + qi] = n > 0 ? top * a.c2 + __builtin_amdgcn_logf(sum) : INFINITY;
   auto finish = [&](auto kept) {                                               // the rows of map m, with what their rounding leaves or without
     const bool second = m == 1;
     const float lam = second ? 0.f : a.lam[h];
@@ -283,13 +283,14 @@ __global__ __launch_bounds__(256) void join_few_kernel(Args a) {
     const f32x4 t = *reinterpret_cast<const f32x4*>(p + s * step + 4 * HD);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      if (t[2 * m + 1] == 0.f) continue;                   // a split without a valid key
+      if (t[2 * m + 1] == 0.f) continue;                   // a split without a key, or of scores of -inf
       const float mx = fmaxf(top[m], t[2 * m]);
       sum[m] = sum[m] * exp2_fast((top[m] - mx) * a.c2) + t[2 * m + 1] * exp2_fast((t[2 * m] - mx) * a.c2);
       top[m] = mx;
     }
   }
   const int qi = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
+  const bool keys = valid_keys(a, b) > 0;
   if (lane * 4 < 2 * HD) {
     f32x4 o[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
     for (int s = 0; s < a.splits; ++s) {
@@ -300,14 +301,14 @@ __global__ __launch_bounds__(256) void join_few_kernel(Args a) {
         o[m] += *reinterpret_cast<const f32x4*>(p + s * step + m * 2 * HD + lane * 4) * exp2_fast((t[2 * m] - top[m]) * a.c2);
       }
     }
-    const f32x4 first = sum[0] == 0.f ? o[0] : o[0] / sum[0], second = sum[1] == 0.f ? o[1] : o[1] / sum[1];
+    const f32x4 first = keys ? o[0] / sum[0] : o[0], second = keys ? o[1] / sum[1] : o[1];
     const int c = h * 2 * HD + lane * 4;
     store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + c, rest_row<HD>(a, 0, b, qi, c), first - second * a.lam[h]);
     if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + c, rest_row<HD>(a, 1, b, qi, c), second);
   }
   if (a.lse && lane < 2) {
     const float s = lane ? sum[1] : sum[0], t = lane ? top[1] : top[0];
-    a.lse[(((int64_t)lane * a.B + b) * a.H + h) * a.Tq + qi] = s == 0.f ? INFINITY : t * a.c2 + __builtin_amdgcn_logf(s);
+    a.lse[(((int64_t)lane * a.B + b) * a.H + h) * a.Tq + qi] = keys ? t * a.c2 + __builtin_amdgcn_logf(s) : INFINITY;
   }
 }
 
@@ -328,7 +329,7 @@ __global__ __launch_bounds__(256) void join_many_kernel(Args a) {
     float top = -INFINITY, sum = 0.f;
     for (int s = lane; s < a.splits; s += 64) {
       const float t = p[s * step + 4 * HD + 2 * m], v = p[s * step + 4 * HD + 2 * m + 1];
-      if (v == 0.f) continue;                                                  // a split without a valid key
+      if (v == 0.f) continue;                                                  // a split without a key, or of scores of -inf
       const float mx = fmaxf(top, t);
       sum = sum * exp2_fast((top - mx) * a.c2) + v * exp2_fast((t - mx) * a.c2);
       top = mx;
@@ -356,6 +357,7 @@ __global__ __launch_bounds__(256) void join_many_kernel(Args a) {
   }
   __syncthreads();
   const int qi = (int)(row % a.Tq), h = (int)(row / a.Tq % a.H), b = (int)(row / a.Tq / a.H);
+  const bool keys = valid_keys(a, b) > 0;
   if (tid < HD / 2) {
     f32x4 first = share[tid], second = share[tid + HD / 2];
 #pragma unroll
@@ -363,13 +365,15 @@ __global__ __launch_bounds__(256) void join_many_kernel(Args a) {
       first += share[q * COLS + tid];
       second += share[q * COLS + tid + HD / 2];
     }
+    if (keys && total[0][1] == 0.f) first *= NAN;                               // 0 / 0 (no split has a weight)
+    if (keys && total[1][1] == 0.f) second *= NAN;
     const int col = h * 2 * HD + tid * 4;
     store4((T*)a.out + (int64_t)b * a.bso + (int64_t)qi * a.ldo + col, rest_row<HD>(a, 0, b, qi, col), first - second * a.lam[h]);
     if (a.out2) store4((T*)a.out2 + ((int64_t)b * a.Tq + qi) * (a.H * 2 * HD) + col, rest_row<HD>(a, 1, b, qi, col), second);
   }
   if (a.lse && tid < 2) {
     const float s = total[tid][1];
-    a.lse[(((int64_t)tid * a.B + b) * a.H + h) * a.Tq + qi] = s == 0.f ? INFINITY : total[tid][0] * a.c2 + __builtin_amdgcn_logf(s);
+    a.lse[(((int64_t)tid * a.B + b) * a.H + h) * a.Tq + qi] = keys ? total[tid][0] * a.c2 + __builtin_amdgcn_logf(s) : INFINITY;
   }
 }
 

@@ -582,7 +582,8 @@ int gpt_add_rmsnorm_bwd(const gpt_add_rmsnorm_bwd_t* a, void* stream);
 
 /* Differential attention: per head two softmax maps of head dim hd over values of 2 hd, and their difference with a learned weight.
  * For batch b, head h, map i = 1, 2 (non-causal, as gpt_attention):
- *   S_i = scale * Q_i K_i^T,  keys >= lengths[b] left out;   P_i = softmax(S_i) over the keys (all 0 where no key is left)
+ *   S_i = scale * Q_i K_i^T,  keys >= lengths[b] left out;   P_i = softmax(S_i) over the keys (all 0 where no key is left; where keys are
+ *   left and every score is -inf it is NaN, as 0 / 0 is)
  *   out = (P_1 - lam[h] P_2) V
  * q, k, v, out: `dtype`; a token holds n_head * 2 * hd elements: head h's are at columns h * 2 hd .. (q and k: map 1's hd, then map
  * 2's).  ld* = elements from token to token, bs* = from sample to sample, so that the three may be column ranges of one fused

@@ -985,3 +985,32 @@ def test_gradients_with_a_graph_are_refused_and_never_constants(T):
         assert all(torch.equal(a, b) and not a.requires_grad for a, b in zip(kept, torch.autograd.grad(out, leaves, g, retain_graph=True)))
         with pytest.raises(RuntimeError, match="differentiated again"):
             torch.autograd.grad(out, leaves, g.requires_grad_(), create_graph=True)
+
+
+@gpu
+@pytest.mark.parametrize("t", [BF, F32])
+@pytest.mark.parametrize("Tq,Tk", [(26, 26), (1, 3), (40, 40), (150, 150), (1, 700), (5, 9000), (600, 2000)])
+def test_diff_attention_rows_of_nothing_but_minus_infinity(Tq, Tk, t):
+    """Scores that are all -inf make their map NaN (0 / 0) at any length - its head's output, dv and that map's dq and dk -, and nothing else:
+    the other map's gradients, the other heads and samples, and a sample without a key (zeros) keep their bits."""
+    B, H, hd = 3, 2, 64
+    _, q, k, v, lam, _, g = attention_case(B, Tq, Tk, H, hd, t, None, False)
+    n = torch.tensor([Tk, 0, Tk], dtype=torch.int32, device=DEV)
+    q.view(B, Tq, H, 2, hd)[0, :, 0, 0, 7] = 1.0
+    runs = []
+    for fill in (0.0, -math.inf):
+        kk = k.clone()
+        kk.view(B, Tk, H, 2, hd)[:2, :, 0, 0, 7] = fill            # head 0, map 0 of sample 0, and of the one without a key
+        leaves = [x.detach().clone().requires_grad_() for x in (q, kk, v, lam)]
+        out = ops.diff_attention(*leaves, H, n)
+        with torch.no_grad():
+            assert torch.equal(ops.diff_attention(*leaves, H, n).nan_to_num(7.0), out.nan_to_num(7.0))
+        runs.append([x.detach() for x in (out, *torch.autograd.grad(out, leaves, g))])
+    (out, dq, dk, dv, dlam), (out0, dq0, dk0, dv0, dlam0) = runs[1], runs[0]
+    assert torch.equal(dlam, dlam0)
+    for got, ref, maps in ((out, out0, False), (dv, dv0, False), (dq, dq0, True), (dk, dk0, True)):
+        got, ref = (x.reshape(B, -1, H, 2, hd) for x in (got, ref))
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[0, :, 0, 0 if maps else slice(None)] = True
+        assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], ref[~hit])
+    assert bool((out[1] == 0).all()) and bool((dq[1] == 0).all()) and bool((dk[1] == 0).all()) and bool((dv[1] == 0).all())
