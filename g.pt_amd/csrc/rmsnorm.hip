@@ -221,6 +221,10 @@ struct Bwd {
   DropoutRng rng;
 };
 
+// rho^3 m, m = mean(w gy x): from m, which is of the order of 1 / rho, up - rho^3 alone leaves the range of fp32 where the rows are below
+// 1e-13 or above 1e13
+__device__ __forceinline__ float cube_scaled(float rho, float m) { return rho * (rho * (rho * m)); }
+
 constexpr int BWD_BLOCKS = 768;  // workgroups at most: rows are dealt out round robin, each keeps its columns' dw sums in registers
 
 // Vector path, one workgroup of W waves per row at a time
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(64 * W) void add_rmsnorm_bwd_kernel(Bwd a) {
       }
     }
     if constexpr (W > 1) __syncthreads();                         // the previous row's sums have been read
-    const float k = rho * rho * rho * (row_sum<W>(s, red) * a.inv_d);
+    const float k = cube_scaled(rho, row_sum<W>(s, red) * a.inv_d);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = lane + LANES * i;
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(256) void add_rmsnorm_bwd_any_kernel(Bwd a) {
       if (part) part[c] = (row == (int64_t)blockIdx.x ? 0.f : part[c]) + gy * (x * rho);
     }
     __syncthreads();
-    const float k = rho * rho * rho * (row_sum<4>(s, red) * a.inv_d);
+    const float k = cube_scaled(rho, row_sum<4>(s, red) * a.inv_d);
     for (int64_t c = threadIdx.x; c < a.d; c += 256) {
       const float x = elem<X>::load(xr + c), gy = elem<H>::load(gyr + c);
       float v = gy * a.w[c] * rho - x * k;

@@ -1014,3 +1014,18 @@ def test_diff_attention_rows_of_nothing_but_minus_infinity(Tq, Tk, t):
         hit[0, :, 0, 0 if maps else slice(None)] = True
         assert bool(got[hit].isnan().all()) and torch.equal(got[~hit], ref[~hit])
     assert bool((out[1] == 0).all()) and bool((dq[1] == 0).all()) and bool((dk[1] == 0).all()) and bool((dv[1] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(5, 520), (3, 37), (2, 8200), (7, 2048)])
+@pytest.mark.parametrize("size", [1e-17, 1e-14, 1e-12, 1e12, 1e14, 1e17])
+def test_rms_norm_gradients_of_small_and_large_rows(size, shape):
+    """The norm does not depend on its rows' size and the gradients are its reciprocal's: as long as the squares are in float32's range the
+    bounds are those of rows around 1 (each scales with the row)."""
+    x, w, gy = normal(1, *shape, std=size).requires_grad_(), (1 + normal(2, shape[-1], std=0.3)).requires_grad_(), normal(3, *shape)
+    y = ops.rms_norm(x, w, 0.0)
+    dx, dw = torch.autograd.grad(y, (x, w), gy)
+    want, tol = norm_reference(None, x.detach(), w.detach(), 0.0, 0.0, 0, 0, gy)
+    within(y, want["y"], tol["y"] + U * (want["y"].abs() + tol["y"]), "y")
+    within(dx, want["dr"], tol["dr"] + U * (want["dr"].abs() + tol["dr"]), "dx")
+    within(dw, want["dw"], tol["dw"], "dweight")
