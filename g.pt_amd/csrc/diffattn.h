@@ -158,8 +158,10 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // ---- tiles shared by a workgroup of NT threads
 // NROWS rows from `src` (row stride ld) by LDS-DMA; rows from `valid` on arrive as zeros (they lie outside the buffer's range).
 // The load is written out because the compiler, which knows the builtin's LDS write, would wait for the tile in flight before every
-// transposing read of the other one.  It has no register result; tile_barrier() waits for it.  (m0, which it sets, is otherwise unused
-// in the kernels that call this: it is the compiler's for LDS-DMA builtins and indexed moves only.)
+// transposing read of the other one.  It has no register result; tile_barrier() waits for it.
+// (A load may read scalar registers that a vector instruction wrote five wait states later at the earliest, and the compiler does not
+// look into the text: the descriptor comes from scalar instructions in every kernel, which tests/test_build_cpu.py checks in the built code; a
+// wait before each tile's loads would cost dK / dV 1 %.)
 template <typename T, int HD, int NROWS, int NT>
 __device__ __forceinline__ void dma_tile(const T* src, int64_t ld, int valid, char* dst, int tid, int wid) {
   using L = Tile<T, HD>;
@@ -184,7 +186,7 @@ __device__ __forceinline__ void dma_tile(const T* src, int64_t ld, int valid, ch
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                      __builtin_amdgcn_readfirstlane((int)(lds + c0 * 16))),
                  "v"(off + more), "s"(rsrc)
-                 : "memory");
+                 : "memory", "m0");
   }
 }
 
@@ -197,7 +199,7 @@ __device__ __forceinline__ void dma_bytes(const void* src, int bytes, char* dst,
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                      __builtin_amdgcn_readfirstlane((int)(uint32_t)(uint64_t)(lds_ptr)dst)),
                  "v"(lane * 16), "s"(rsrc)
-                 : "memory");
+                 : "memory", "m0");
 }
 
 // this lane's row of 32 in a tile, as the base that Tile::add takes with an even chunk number C (the lane half reads chunk C + hh)
