@@ -82,3 +82,29 @@ def test_loads_to_lds_wait_for_their_descriptors(tmp_path):
         loads += n
         assert not bad, (code, bad[:3])
     assert loads > 500
+
+
+def included(name, seen=None):
+    """The headers of this folder and the C interface that a source reads, through other headers too."""
+    seen = set() if seen is None else seen
+    for path in re.findall(r'#include "([^"]+)"', open(os.path.join(CSRC, name)).read()):
+        if path not in seen:
+            seen.add(path)
+            included(path, seen)
+    return seen
+
+
+def would_build(*args):
+    """The commands of a make that thinks these files have changed."""
+    return subprocess.run(["make", "-n", "-C", CSRC, *args], check=True, capture_output=True, text=True).stdout
+
+
+def test_a_changed_header_rebuilds_every_object_that_reads_it():
+    sources = [n for n in os.listdir(CSRC) if n.endswith((".hip", ".cpp")) and n != "ops_binding.cpp"]
+    headers = {h for n in sources for h in included(n)}
+    assert {"philox.h", "short_tiles.h", "../../include/gpt_hip.h"} <= headers
+    for header in headers:
+        built = would_build("-W", header)
+        for n in sources:
+            if header in included(n):
+                assert re.search(rf" -c {re.escape(n)} ", built), (header, n)
