@@ -108,3 +108,20 @@ def test_a_changed_header_rebuilds_every_object_that_reads_it():
         for n in sources:
             if header in included(n):
                 assert re.search(rf" -c {re.escape(n)} ", built), (header, n)
+
+
+def test_another_torch_rebuilds_the_binding(tmp_path):
+    """The binding is compiled against torch's headers: one built for the torch that is there is kept, another torch makes a new one.  The
+    compiler is a script that notes its runs, the torch a folder with a version."""
+    compiler, runs, binding = tmp_path / "cxx", tmp_path / "runs", str(tmp_path / "gpt_ops.so")
+    compiler.write_text(f'#!/bin/sh\necho run >> {runs}\nwhile [ "$1" != -o ]; do shift; done\necho built > "$2"\n')
+    compiler.chmod(0o755)
+    (tmp_path / "torch").mkdir()
+    (tmp_path / "torch" / "__init__.py").write_text("")
+
+    def make(version):
+        (tmp_path / "torch" / "version.py").write_text(f"__version__ = {version!r}\n")
+        subprocess.run(["make", "-C", CSRC, binding, "BIND=" + binding, f"CXX={compiler}", f"PYTHON=env PYTHONPATH={tmp_path} python3"], check=True,
+                       capture_output=True)
+        return len(runs.read_text().split())
+    assert [make(v) for v in ("1", "1", "2", "2", "1")] == [1, 1, 2, 2, 3]
