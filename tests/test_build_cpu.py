@@ -125,3 +125,11 @@ def test_another_torch_rebuilds_the_binding(tmp_path):
                        capture_output=True)
         return len(runs.read_text().split())
     assert [make(v) for v in ("1", "1", "2", "2", "1")] == [1, 1, 2, 2, 3]
+
+
+def test_the_c_library_needs_no_torch():
+    without = "PYTHON=python3 -I -S"                                     # no site-packages, so no torch
+    for args in (["lib"], ["all", without], [without]):
+        listed = would_build(*args, "-B")
+        assert "-o ../lib/libgpt_hip.so" in listed and "ops_binding.cpp" not in listed, args
+    assert "ops_binding.cpp" in would_build("-B")
