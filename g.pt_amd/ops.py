@@ -7,7 +7,9 @@
 
 All take GPU tensors, run on the current stream of the tensors' device, allocate only their results (and a scratch buffer of their
 own), never synchronise, and can be captured into a HIP graph.  The floating-point ones differentiate (once) through torch.autograd;
-their gradients do not change from run to run.  There is no CPU fallback: what the kernels do not take raises GptHipError.
+their gradients do not change from run to run.  bfloat16 results are those of float32 arithmetic, rounded once.  There is no CPU
+fallback: what the kernels do not take raises GptHipError, and so do forward-mode differentiation, tracing (jit.trace, make_fx, fake
+tensors) and the transforms of torch.func; gradients of gradients raise in the backward pass.
 
 Tensors used on another stream than the one they were made on: as everywhere in torch, the caller orders the streams (and calls
 record_stream where an input may be freed early).  Capturing a backward pass into a graph: warm the step up on a side stream first
@@ -41,8 +43,9 @@ def dropout_add(h, resid, p, seed, offset=0, counter=None):
 
     The mask is a function of (seed, offset, element index): the same pair gives the same mask, so every site of a step takes an
     offset of its own.  `counter`: an int64 GPU tensor of one element that is added to `offset` when the kernel runs; a captured
-    step that advances it between replays draws new masks (it must not change between a forward and its backward).  p is realised
-    in steps of 1/65536; kept values are scaled by 1 / (1 - p)."""
+    step that advances it between replays draws new masks (it must not change between a forward and its backward).  Advance it by the
+    number of offsets that a step uses, at least: with sites at offsets 0 .. n - 1 and an advance of less than n, a site draws masks that
+    another site drew a step before.  p is realised in steps of 1/65536; kept values are scaled by 1 / (1 - p)."""
     if resid is None:
         raise L.GptHipError("dropout_add: resid is None (use dropout)")
     return (_host or _load()).dropout_add(h, resid, p, seed & _U64, offset & _U64, counter)

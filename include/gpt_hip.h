@@ -517,7 +517,8 @@ int gpt_pack_tensors_if_changed(const gpt_pack_item_t* items, int n_items, int64
  * 65536 / (65536 - thr): p is realised in steps of 1 / 65536 and the expectation is exact for the realised one (p = 1: all dropped).
  * Same (seed, offset) = same mask: give every site of a step its own offset.  offset_dev: a device counter (or NULL) added to
  * offset, read by the kernel - a captured graph whose replays advance it draws new masks; forward and backward of a step must find
- * the same value there. */
+ * the same value there.  Advance it per step by the number of offsets that a step uses, at least: by less, and a site draws the masks that
+ * another site drew a step before. */
 typedef struct {
   double p;
   uint64_t seed, offset;
@@ -640,7 +641,8 @@ int gpt_attention_dropout_bwd(int dtype, const void* qkv, const void* dy, void* 
 
 /* The probabilities of transformer.py:34-72, 302-314 (embd: position-embedded tokens; attn: attention probabilities; resid: the
  * outputs of both residual branches of a Block).  The masks of a step take the offsets offset .. offset + 3 n_layer: site 0 = embd,
- * 1 + 3 l, 2 + 3 l, 3 + 3 l = Block l's attention, projection and MLP; forward and backward of a step are given the same struct.
+ * 1 + 3 l, 2 + 3 l, 3 + 3 l = Block l's attention, projection and MLP; forward and backward of a step are given the same struct.  A device
+ * counter therefore advances by 3 n_layer + 1 per step at least.
  * (GPT_BF16 with d % 256 == 0: the last Block works on the decoded tokens' rows alone and its two residual masks are those of the compact
  * rows, in the training forward as in the one without kept activations.) */
 typedef struct {

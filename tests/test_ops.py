@@ -1029,3 +1029,35 @@ def test_rms_norm_gradients_of_small_and_large_rows(size, shape):
     within(y, want["y"], tol["y"] + U * (want["y"].abs() + tol["y"]), "y")
     within(dx, want["dr"], tol["dr"] + U * (want["dr"].abs() + tol["dr"]), "dx")
     within(dw, want["dw"], tol["dw"], "dweight")
+
+
+@gpu
+def test_dropout_counter_advances_by_the_offsets_of_a_step():
+    """Sites at offsets 0 .. 2 of a captured step: advanced by three per replay, no mask comes twice; by one (too little, as the documentation
+    says), a site draws what its neighbour drew a step before."""
+    sites, steps = 3, 4
+    h = torch.ones(64, 96, device=DEV)
+    counter = torch.zeros(1, dtype=torch.int64, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.dropout(h, 0.5, 21, 0, counter)
+    torch.cuda.current_stream().wait_stream(side)
+    for advance in (sites, 1):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            masks = [ops.dropout(h, 0.5, 21, s, counter) for s in range(sites)]
+            counter.add_(advance)
+        counter.zero_()
+        seen = []
+        for step in range(steps):
+            graph.replay()
+            torch.cuda.synchronize()
+            seen.append([m.clone() for m in masks])
+            assert all(torch.equal(m, ops.dropout(h, 0.5, 21, s + advance * step)) for s, m in enumerate(seen[-1]))
+        flat = [m for step in seen for m in step]
+        same = [(i, j) for i in range(len(flat)) for j in range(i) if torch.equal(flat[i], flat[j])]
+        if advance == sites:
+            assert not same
+        else:
+            assert torch.equal(seen[1][0], seen[0][1]) and torch.equal(seen[1][1], seen[0][2])
