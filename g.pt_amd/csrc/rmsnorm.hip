@@ -39,6 +39,7 @@ struct Fwd {
   int64_t ldh, ldr, ldx, ldy, rows, d;
   float eps, inv_d;
   DropoutRng rng;
+  int64_t first;                // row of this launch's first workgroup
 };
 
 __device__ __forceinline__ float4 sq4(const float (&v)[8]) {
@@ -68,7 +69,7 @@ __global__ __launch_bounds__(64 * W) void add_rmsnorm_kernel(Fwd a) {
   __shared__ float red[W];
   constexpr int LANES = 64 * W;
   const int lane = threadIdx.x;
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const int n8 = (int)(a.d >> 3);
   const X* rr = (const X*)a.resid + row * a.ldr;
   float x[NC][8];
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(64 * W) void add_rmsnorm_kernel(Fwd a) {
 template <typename H, typename X, bool MX>
 __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(Fwd a) {
   __shared__ float red[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const X* rr = (const X*)a.resid + row * a.ldr;
   const uint64_t off = a.rng.thr ? dropout_offset(a.rng) : 0;
   const X* src = rr;
@@ -191,23 +192,24 @@ __global__ __launch_bounds__(256) void add_rmsnorm_any_kernel(Fwd a) {
   }
 }
 
+constexpr int64_t LAUNCH_ROWS = 1 << 23;   // a workgroup per row: a grid of at most 2^32 threads
+
 template <typename H, typename X, bool MX>
-int launch_fwd(const Fwd& a, bool vec, hipStream_t s) {
-  if (!vec || a.d > 8192) {
-    GPT_REQUIRE(a.rows < (1ll << 24), "gpt_add_rmsnorm: %lld rows exceed this path's grid", (long long)a.rows);
-    hipLaunchKernelGGL((add_rmsnorm_any_kernel<H, X, MX>), dim3((unsigned)a.rows), dim3(256), 0, s, a);
-    return gpt_launch_status("gpt_add_rmsnorm");
-  }
-  GPT_REQUIRE(a.rows < (1ll << 24), "gpt_add_rmsnorm: too many rows (%lld)", (long long)a.rows);
-#define RN(NC, W) hipLaunchKernelGGL((add_rmsnorm_kernel<H, X, MX, NC, W>), dim3((unsigned)a.rows), dim3(64 * W), 0, s, a)
-  if (a.d <= 512) RN(1, 1);
-  else if (a.d <= 1024) RN(1, 2);
-  else if (a.d <= 1536) RN(1, 3);
-  else if (a.d <= 2048) RN(1, 4);
-  else if (a.d <= 4096) RN(2, 4);
-  else RN(4, 4);
+int launch_fwd(Fwd a, bool vec, hipStream_t s) {
+  for (a.first = 0; a.first < a.rows; a.first += LAUNCH_ROWS) {
+    const dim3 grid((unsigned)(a.rows - a.first < LAUNCH_ROWS ? a.rows - a.first : LAUNCH_ROWS));
+#define RN(NC, W) hipLaunchKernelGGL((add_rmsnorm_kernel<H, X, MX, NC, W>), grid, dim3(64 * W), 0, s, a)
+    if (!vec || a.d > 8192) hipLaunchKernelGGL((add_rmsnorm_any_kernel<H, X, MX>), grid, dim3(256), 0, s, a);
+    else if (a.d <= 512) RN(1, 1);
+    else if (a.d <= 1024) RN(1, 2);
+    else if (a.d <= 1536) RN(1, 3);
+    else if (a.d <= 2048) RN(1, 4);
+    else if (a.d <= 4096) RN(2, 4);
+    else RN(4, 4);
 #undef RN
-  return gpt_launch_status("gpt_add_rmsnorm");
+    if (int st = gpt_launch_status("gpt_add_rmsnorm")) return st;
+  }
+  return 0;
 }
 
 // ---------------------------------------------------------------------------------------------------------------- backward
@@ -392,7 +394,7 @@ extern "C" int gpt_add_rmsnorm(const gpt_add_rmsnorm_t* p, void* stream) {
   GPT_REQUIRE(elem_aligned(p->h, hs) && elem_aligned(p->resid, xs) && elem_aligned(p->x_out, xs) && elem_aligned(p->weight, 4) &&
                   elem_aligned(p->y, ys) && elem_aligned(p->rho, 4),
               "%s: misaligned element", who);
-  Fwd a{p->h, p->resid, p->x_out, p->y, p->weight, p->scales, p->rho, p->ldh, p->ldr, p->ldx, p->ldy, p->rows, p->d, p->eps, 1.0f / (float)p->d, {}};
+  Fwd a{p->h, p->resid, p->x_out, p->y, p->weight, p->scales, p->rho, p->ldh, p->ldr, p->ldx, p->ldy, p->rows, p->d, p->eps, 1.0f / (float)p->d, {}, 0};
   if (int st = gpt_dropout_rng(p->drop, &a.rng, who)) return st;
   const bool vec = p->d % 8 == 0 && rows_aligned16(p->resid, p->ldr, xs) && aligned16(p->weight) &&
                    (!p->h || (rows_aligned16(p->h, p->ldh, hs) && rows_aligned16(p->x_out, p->ldx, xs))) &&

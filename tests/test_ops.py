@@ -1061,3 +1061,30 @@ def test_dropout_counter_advances_by_the_offsets_of_a_step():
             assert not same
         else:
             assert torch.equal(seen[1][0], seen[0][1]) and torch.equal(seen[1][1], seen[0][2])
+
+
+@gpu
+@pytest.mark.parametrize("d", [8, 5])
+def test_rms_norm_of_more_rows_than_a_grid_takes(d):
+    """2^24 rows and some (a norm over every head has that many): both halves and the last rows are what few rows give, with their masks."""
+    rows, p = (1 << 24) + 5, 0.3
+    some = torch.cat([torch.arange(3), (1 << 23) + torch.arange(-2, 3), (1 << 24) + torch.arange(-2, 5)]).to(DEV)
+    h, r = torch.empty(rows, d, dtype=BF, device=DEV), torch.ones(rows, d, device=DEV)
+    h[:], w = torch.arange(d, device=DEV) + 1, 1 + normal(3, d, std=0.3)
+    h[some] = normal(1, len(some), d, dtype=BF)
+    r[some] = normal(2, len(some), d)
+    h.requires_grad_()
+    y, x = ops.add_rms_norm(h, r, w, 1e-5, p, 5, 6)
+    gy = torch.zeros_like(y)
+    gy[some] = normal(4, len(some), d, dtype=BF)
+    dh, = torch.autograd.grad(y, h, gy)
+    for row in some.tolist():
+        base = (row * d) // 8 * 8
+        keep = philox_keep(row * d - base + d, p, 5, 6, base)[row * d - base:].to(DEV)
+        want = r[row] + torch.where(keep, h.detach()[row].float() * factor(p), 0.0)
+        assert torch.equal(x[row], want), row
+        ref, tol = norm_reference(None, want[None], w, 1e-5, 0.0, 0, 0, gy[row][None])
+        within(y[row][None], ref["y"], tol["y"] + HALF[BF] * (ref["y"].abs() + tol["y"]), "y")
+        dhr, t = torch.where(keep, ref["dr"] * factor(p), 0.0), torch.where(keep, (tol["dr"] + U * ref["dr"].abs()) * factor(p), 0.0)
+        within(dh[row][None], dhr, t + HALF[BF] * (dhr.abs() + t), "dh")
+    assert bool(torch.isfinite(y[:: 1 << 20]).all())
