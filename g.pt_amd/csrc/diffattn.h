@@ -26,7 +26,7 @@ struct Args {
   void *dq, *dk, *dv;
   int64_t lddq, bsdq, lddk, bsdk, lddv, bsdv;
   const f32x4* stats;         // [B][H][Tq]: lse_1, lse_2, D_1, D_2
-  float* dlam_part;           // [H][B * splits * key tiles]
+  float* dlam_part;           // [H][B * splits * key tiles], fp32 [H][B * query tiles]
   // split sweeps: spans of q_tiles / k_tiles tiles of 32, sums of a span [span][B * H][Tq or Tk][2 hd]
   int q_splits, q_tiles, k_splits, k_tiles;
   float *dq_part, *dk_part, *dv_part;

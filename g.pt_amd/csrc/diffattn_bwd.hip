@@ -3,7 +3,9 @@
 //   dQ_i = c dS_i K_i,  dK_i = c dS_i^T Q_i,  dV = (P_1 - lam P_2)^T dO,  dlam = -sum P_2 dP
 // The maps are recomputed from the kept log-sum-exps; D_i = dO . O_i comes from the kept outputs. Two sweeps, over key tiles for dQ
 // and over query tiles for dK / dV, so that every sum is taken by one wave in a fixed order (or by one per span, joined in the spans'
-// order); dlam is summed from the fp32 P_2 and dP of the second sweep (from the rounded outputs it would carry their rounding error).
+// order).  dlam, which is what nearly cancelling terms leave: in bf16 from the fp32 P_2 and dP of the second sweep (D_2 is good to 16 bits); in
+// fp32 the sum of the rows' D_2, whose maps the forward has divided by their own sums (a row of recomputed P_2 adds to 1 within the
+// rounding of its log-sum-exp, some 4e-7: 4 x 257 tokens up to 1.2e-6 of dlam off, the plain formula in fp32 6e-7).
 // A wave holds 16 rows of its side for BOTH maps - operands and accumulators, some 230 registers at hd 128, two waves per SIMD: dP
 // serves both maps, so a wave per map would compute it twice (a third more matrix work in dQ, a half in dK / dV), and 32 rows per wave
 // would leave one wave per SIMD with nothing beside it while it waits for LDS or exponentials (T = 4096, 16 (sample, head), hd 128, with
@@ -326,6 +328,10 @@ __global__ __launch_bounds__(NW * 64) void dq_kernel(Args a) {
     now = next;
   }
   if (late && n > 0) products(before);
+  if constexpr (sizeof(T) == 4) {
+    const float sum = wave_sum(qok && g == 0 ? st[3] : 0.f);
+    if (lane == 0 && split == 0) a.dlam_part[((int64_t)h * a.B + b) * (blocks * NW) + block * NW + wid] = sum;
+  }
   if (!qok) return;
   auto store = [&](auto* dq) {
 #pragma unroll
@@ -341,6 +347,7 @@ template <typename T, int HD, int NW>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HD == 64 ? 3 : 1) void dkv_kernel(Args a) {
   using L = Tile<T, HD>;
   constexpr int NT = NW * 64, NS = STAGES<T, NW>, TILE = 32 * L::PITCH, STAGE = 2 * TILE + 512, KC = HD / 32, CT = HD / 16;
+  constexpr bool NEGATE = sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];            // [NS][Q | dO | stats]
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -363,12 +370,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HD == 64 ? 3 : 1) void d
     for (int c = 0; c < 2 * KC; ++c) {
       kf[c] = frag_row(kr, c, g, ok);
       vf[c] = frag_row(vr, c, g, ok);
-      if (wid & 1) frag_negate(vf[c]);
+      if (NEGATE && wid & 1) frag_negate(vf[c]);
     }
   }
-  // The matrix unit's sums lean down by some 2^-32 of their terms' size: next to nothing, but dlam is what nearly cancelling terms leave
-  // (at 4 x 4096 x 4096 of them the lean is 1e-6 of it).  Every other wave takes -V and so has the lean of -dP.
-  const float sign = wid & 1 ? -1.f : 1.f;
+  // The matrix unit's sums lean down by some 2^-32 of their terms' size: next to nothing, but dlam's terms nearly cancel (at 4 x 4096 x
+  // 4096 of them the lean is 1e-6 of it).  Where it is summed here every other wave takes -V and so has the lean of -dP.
+  const float sign = NEGATE && wid & 1 ? -1.f : 1.f;
   const float lam = a.lam[h];
   f32x4 dk[2 * CT], dv[2 * CT];
 #pragma unroll
@@ -418,11 +425,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HD == 64 ? 3 : 1) void d
         const float p0 = exp2_fast(s[0][u][r] * a.c2 - st[0]), p1 = exp2_fast(s[1][u][r] * a.c2 - st[1]);
         const float d = sign * dp[u][r];
         p[u][r] = p0 - lam * p1;
-        part += p1 * d;
+        if constexpr (sizeof(T) == 2) part += p1 * d;
         s[0][u][r] = p0 * (d - st[2]);
         s[1][u][r] = p1 * (d - st[3]);                                       // -lam: at the end, once
       }
-    dlam += opaque(part);                                                    // here, not behind the products: its terms would be kept over them
+    if constexpr (sizeof(T) == 2) dlam += opaque(part);                                                    // here, not behind the products: its terms would be kept over them
     frag_pair(pf, pl, p[0], p[1]);
 #pragma unroll
     for (int m = 0; m < 2; ++m) frag_pair(df[m], dl[m], s[m][0], s[m][1]);
@@ -461,8 +468,10 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && HD == 64 ? 3 : 1) void d
   }
   if (late && n > 0) products(before);
   // a masked key's lane has computed with zeros for its operands and another row's statistics: it gives zeros
-  const float sum = wave_sum(ok ? (float)dlam : 0.f);
-  if (lane == 0) a.dlam_part[(((int64_t)h * a.B + b) * a.q_splits + split) * (blocks * NW) + block * NW + wid] = sum;
+  if constexpr (sizeof(T) == 2) {
+    const float sum = wave_sum(ok ? (float)dlam : 0.f);
+    if (lane == 0) a.dlam_part[(((int64_t)h * a.B + b) * a.q_splits + split) * (blocks * NW) + block * NW + wid] = sum;
+  }
   if (key >= a.Tk) return;
   auto store = [&](auto* dkr, auto* dvr) {
     const f32x4 none = {0.f, 0.f, 0.f, 0.f};
@@ -561,7 +570,8 @@ Plan plan_for(int dtype, int B, int Tq, int Tk, int H, int hd) {
   if (!p.many_k) spans(pairs * ((kt + 1) / 2), fill, qt, least, &p.q_splits, &p.q_tiles);
   if (!p.many_q) spans(pairs * ((qt + 1) / 2), fill, kt, least, &p.k_splits, &p.k_tiles);
   p.stats = 16 * pairs * Tq;
-  p.dlam = round16(pairs * p.q_splits * (((int64_t)Tk + 127) / 128 * 8) * 4);   // one per 16 keys of the workgroups' blocks
+  // one per 16 keys of the workgroups' blocks and span, in fp32 one per 16 queries
+  p.dlam = round16((dtype == GPT_BF16 ? pairs * p.q_splits * (((int64_t)Tk + 127) / 128 * 8) : pairs * (((int64_t)Tq + 127) / 128 * 8)) * 4);
   p.dq = p.k_splits > 1 ? pairs * p.k_splits * Tq * 2 * hd * 4 : 0;
   p.dkv = p.q_splits > 1 ? pairs * p.q_splits * Tk * 2 * hd * 4 : 0;
   return p;
@@ -599,8 +609,9 @@ int launch(const Args& a, const Plan& plan, f32x4* stats, float* dlam, hipStream
   constexpr int M = MANY<T, HD>, MK = MANY_KEYS<T, HD>;
   if (int st = plan.many_k ? launch_dkv<T, HD, MK>(a, s) : launch_dkv<T, HD, FEW>(a, s)) return st;
   if (int st = plan.many_q ? launch_dq<T, HD, M>(a, s) : launch_dq<T, HD, FEW>(a, s)) return st;
-  const int nk = plan.many_k ? MK : FEW;
-  const int64_t parts = (int64_t)a.B * a.q_splits * (((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk);
+  const int nk = plan.many_k ? MK : FEW, nq = plan.many_q ? M : FEW;                    // parts of dlam per head
+  const int64_t parts = sizeof(T) == 2 ? (int64_t)a.B * a.q_splits * (((int64_t)a.Tk + 16 * nk - 1) / (16 * nk) * nk)
+                                       : (int64_t)a.B * (((int64_t)a.Tq + 16 * nq - 1) / (16 * nq) * nq);
   const int64_t joined = ((a.k_splits > 1 ? rows : 0) + (a.q_splits > 1 ? 2 * pairs * a.Tk : 0)) * (HD / 2);
   if (joined > 0)
     hipLaunchKernelGGL((join_kernel<T, HD>), dim3((unsigned)(a.H + (joined + 255) / 256)), dim3(256), 0, s, a, parts, dlam);
