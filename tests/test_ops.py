@@ -1088,3 +1088,76 @@ def test_rms_norm_of_more_rows_than_a_grid_takes(d):
         dhr, t = torch.where(keep, ref["dr"] * factor(p), 0.0), torch.where(keep, (tol["dr"] + U * ref["dr"].abs()) * factor(p), 0.0)
         within(dh[row][None], dhr, t + HALF[BF] * (dhr.abs() + t), "dh")
     assert bool(torch.isfinite(y[:: 1 << 20]).all())
+
+
+@gpu
+@pytest.mark.parametrize("B,T,H,t", [(3, 26, 2, BF), (2, 150, 2, BF), (1, 600, 1, BF), (2, 150, 2, F32)])
+def test_a_captured_training_pass(B, T, H, t):
+    """Forward and backward of norm, attention and dropout in one graph, warmed up on a side stream as the documentation says: every replay, with
+    other data in the same buffers and eager passes between, is the eager pass."""
+    hd = 64
+    w = 2 * H * hd
+    data = [[normal(10 * s + i, B, T, n, dtype=d) for i, (n, d) in enumerate(((w, t), (w, F32), (3 * w, t), (w, t), (w, F32)))] for s in range(3)]
+    lens = torch.tensor(([T, T - 3, 1] * B)[:B], dtype=torch.int32, device=DEV)
+    weight, lam = 1 + normal(90, w, std=0.2), 0.5 + normal(91, H, std=0.2)
+
+    def step(h, x, qkv, gy, gx):
+        leaves = [v.requires_grad_() for v in (h, x, qkv, weight, lam)]
+        a = ops.diff_attention_qkv(qkv, lam, H, lens)
+        y, s = ops.add_rms_norm(a + h, x, weight, p=0.2, seed=3, offset=1)
+        s = ops.dropout_add(y, s, 0.1, 3, 2)
+        return [v.detach() for v in (y, s, *torch.autograd.grad((y, s), leaves, (gy, gx)))]
+
+    fresh = lambda d: [v.clone() for v in d]                                                                 # noqa: E731
+    want = [step(*fresh(d)) for d in data]
+    static = fresh(data[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(*static)
+    for i in (0, 1, 2, 1, 0):
+        with torch.no_grad():
+            for dst, src in zip(static, data[i]):
+                dst.copy_(src)
+        graph.replay()
+        other = step(*fresh(data[(i + 1) % 3]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i])), i
+        assert all(torch.equal(a, b) for a, b in zip(other, want[(i + 1) % 3])), i
+
+
+@gpu
+def test_two_threads_at_once():
+    """Calls and backward passes from two Python threads on streams of their own: each thread's results are the ones it gets alone."""
+    import threading
+    work = []
+    for s, T in ((1, 26), (2, 300)):
+        qkv, lam, g = normal(s, 2, T, 384, dtype=BF).requires_grad_(), torch.rand(1, device=DEV).requires_grad_(), normal(s + 5, 2, T, 128, dtype=BF)
+        work.append((qkv, lam, g))
+
+    def run(qkv, lam, g):
+        out = ops.diff_attention_qkv(qkv, lam, 1)
+        return [out.detach(), *torch.autograd.grad(out, (qkv, lam), g)]
+
+    want = [run(*x) for x in work]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def thread(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(run(*work[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:                                                                               # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in (0, 1)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not failed and all(len(x) == 20 for x in got)
+    assert all(torch.equal(a, b) for i in (0, 1) for r in got[i] for a, b in zip(r, want[i]))
