@@ -11,8 +11,8 @@
 // bf16: P enters the second product as two operands, its rounding to bf16 and what that left (16 bits of mantissa), so that the output's
 // own rounding is the only one to 8 bits.  One operand alone leaves the output 2.55e-3 rms off at 4096 keys where rounding the exact
 // result leaves 1.66e-3 (the maps' difference cancels values, not their noise).  The second costs nothing where memory is the bound (one
-// query group) and, where the matrix unit is, half of its work again: 2 x 4096 tokens, 8 heads, hd 128, 560 us (1.23 PFLOP/s of its 687
-// GFLOP) instead of 406, 16 samples of up to 515 tokens, hd 64, 50 instead of 44.
+// query group) and, where the matrix unit is, half of its work again: 2 x 4096 tokens, 8 heads, hd 128, 563 us (1.22 PFLOP/s of its 687
+// GFLOP) instead of 407, 16 samples of up to 515 tokens, hd 64, with what is kept for the backward, 53 instead of 44.
 // The accumulator is rescaled only when a row's maximum has grown by more than a factor of 2^8 over the reference its sums are held
 // against: P stays below 2^8.
 #include "diffattn.h"

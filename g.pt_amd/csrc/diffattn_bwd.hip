@@ -5,7 +5,7 @@
 // and over query tiles for dK / dV, so that every sum is taken by one wave in a fixed order (or by one per span, joined in the spans'
 // order).  dlam, which is what nearly cancelling terms leave: in bf16 from the fp32 P_2 and dP of the second sweep (D_2 is good to 16 bits); in
 // fp32 the sum of the rows' D_2, whose maps the forward has divided by their own sums (a row of recomputed P_2 adds to 1 within the
-// rounding of its log-sum-exp, some 4e-7: 4 x 257 tokens up to 1.2e-6 of dlam off, the plain formula in fp32 6e-7).
+// rounding of its log-sum-exp: 40 draws of 4 x 257 tokens 6.3e-7 of dlam off rms, from D_2 4.8e-7, the plain formula in fp32 5.5e-7).
 // A wave holds 16 rows of its side for BOTH maps - operands and accumulators, some 230 registers at hd 128, two waves per SIMD: dP
 // serves both maps, so a wave per map would compute it twice (a third more matrix work in dQ, a half in dK / dV), and 32 rows per wave
 // would leave one wave per SIMD with nothing beside it while it waits for LDS or exponentials (T = 4096, 16 (sample, head), hd 128, with
@@ -13,8 +13,8 @@
 // by the workgroup's waves; every tile is used twice, by rows for the scores and transposed for the gradient products.
 // bf16: P and dS enter the gradient products as two operands each (16 bits of mantissa), so that the gradients' own rounding is the
 // only one to 8 bits: one operand leaves dQ, dK, dV 2.35e-3 rms off where rounding the exact result leaves 1.66e-3.  It costs half of
-// dK / dV's matrix work again and a third of dQ's: 737 and 521 us (1.12 and 1.06 PFLOP/s of their 824 and 550 GFLOP) instead of 640 and
-// 470; 16 samples of up to 515 tokens, hd 64, 57 and 46 instead of 47 and 39.
+// dK / dV's matrix work again and a third of dQ's: 757 and 538 us (1.09 and 1.02 PFLOP/s of their 824 and 550 GFLOP) instead of 640 and
+// 471; 16 samples of up to 515 tokens, hd 64, 53 and 44 instead of 47 and 39.
 #include "diffattn.h"
 
 namespace diffattn {

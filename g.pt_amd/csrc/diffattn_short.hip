@@ -12,7 +12,7 @@
 // bf16: P and dS enter their products as two operands each (16 bits of mantissa; the values are exact products of them), so the
 // results' own rounding is the only one to 8 bits.  HBM-bound, which is why that costs little: the backward reads 4 row sets of Tq or
 // Tk x 2 hd and writes 3 for some 2 MFLOP each, the forward 3 and 1.  1024 samples x 26 tokens, 8 heads of 2 x 96, bf16: forward
-// 74 us (64 at a copy's rate), backward 130 (111; 124 with one operand, whose dQ, dK, dV are off by 2.35e-3 rms instead of
+// 74 us (64 at a copy's rate), backward 133 (111; 124 with one operand, whose dQ, dK, dV are off by 2.35e-3 rms instead of
 // 1.66e-3); 64 samples forward 7.6.
 #include "short_tiles.h"
 

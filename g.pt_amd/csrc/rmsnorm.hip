@@ -2,7 +2,7 @@
 //   x = resid + drop(h),  rho = (mean x^2 + eps)^-1/2,  y = x rho w            (stands beside layernorm_kernel of norm.hip)
 //   dx = gx + rho (w gy) - x rho^3 mean(w gy x),  dresid = dx,  dh = drop(dx),  dw = sum_rows gy x rho
 // HBM-bound: every operand once.  A row stays in registers between its sum and its use; the mask is drawn again in the backward.
-// 13312 x 2048, bf16 h and y, fp32 stream: forward 59 us (327 MB, 5.5 TB/s), backward 85 (436 MB, 5.1) and 4 for dw's partial rows;
+// 13312 x 2048, bf16 h and y, fp32 stream: forward 59 us (327 MB, 5.5 TB/s), backward 84 (436 MB, 5.2) and 5 for dw's partial rows;
 // 8320 x 1536 to 8 bits 27 us (141 MB, 5.2).
 #include "philox.h"
 
