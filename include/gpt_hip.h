@@ -590,8 +590,8 @@ int gpt_add_rmsnorm_bwd(const gpt_add_rmsnorm_bwd_t* a, void* stream);
  * 2's).  ld* = elements from token to token, bs* = from sample to sample, so that the three may be column ranges of one fused
  * [B * T, 3 * n_head * 2 * hd] projection.  hd 32, 64, 96 or 128; rows 16-byte aligned.  lam: fp32 [n_head].  lengths: int32
  * device [B] or NULL (all Tk); values outside [0, Tk] are clamped; what lies in k and v behind a sample's length is never read into
- * the result (NaN included).  1 <= Tq, Tk <= 2^24 (the backward: B * n_head * Tq < 2^28).  ws: gpt_diff_attention_workspace() bytes of scratch, 16-byte aligned (0 bytes: may
- * be NULL); calls that overlap in time need a ws each.
+ * the result (NaN included).  1 <= Tq, Tk <= 2^24 (the backward: B * n_head * Tq < 2^28).  ws: gpt_diff_attention_workspace() bytes of
+ * scratch, 16-byte aligned (0 bytes: may be NULL); calls that overlap in time need a ws each.
  * For the backward, keep: lse (fp32 [2][B][n_head][Tq], the maps' base-2 log-sum-exp) and out2 (`dtype` [B][Tq][n_head * 2 * hd],
  * the second map's P_2 V); both NULL where no gradient is wanted, and where Tq and Tk are both <= 32: that backward recomputes the
  * maps from q and k and needs neither them nor out. */
